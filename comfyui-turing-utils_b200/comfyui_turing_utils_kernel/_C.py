@@ -8,12 +8,13 @@ device (the reference's TorchOpContext, bindings.cpp:17-31).
 """
 from __future__ import annotations
 
+import ctypes
 import math
 
 import torch
 
 from . import _lib
-from ._lib import call, float_dtype_code, ptr, stream_of
+from ._lib import POSITION_TYPES, call, float_dtype_code, layout_strides, ptr, stream_of
 
 
 def _check(cond: bool, msg: str) -> None:
@@ -554,4 +555,99 @@ def turing_layer_norm_adaln(input, scale, shift, epsilon):
         call("tb_layer_norm_adaln", ptr(input), ptr(scale), ptr(shift), ptr(out), input.size(0),
              input.size(1), input.size(2), scale.size(1), float_dtype_code(input), float(epsilon),
              stream_of(input))
+    return out
+
+
+# ----------------------------------------------------------- rotary positions
+
+def _rope_positions(positions, inv_freq, axis_pairs, batch, length, device):
+    """Checks the positions and frequencies of a rotary call; returns them as the
+    kernel reads them with the number of position rows, the axes and their pairs."""
+    _check(positions.is_cuda and inv_freq.is_cuda and positions.device == device
+           and inv_freq.device == device,
+           "rotary positions and frequencies must use the input's CUDA device")
+    _check(positions.dtype in POSITION_TYPES,
+           "positions must be int32, int64, float32, or float64")
+    _check(inv_freq.dim() == 1 and inv_freq.numel() > 0
+           and inv_freq.dtype in (torch.float32, torch.float64),
+           "inv_freq must be a 1D float32 or float64 tensor")
+    axes = 1 if axis_pairs is None else len(axis_pairs)
+    _check(1 <= axes <= 4, "positions must have 1 to 4 axes")
+    _check(axis_pairs is None or (min(axis_pairs) >= 0 and sum(axis_pairs) == inv_freq.numel()),
+           "axis_pairs must add up to the number of channel pairs")
+    if axis_pairs is None:
+        positions = positions.unsqueeze(-1)
+    if positions.dim() == 2:
+        positions = positions.unsqueeze(0)
+    _check(positions.dim() == 3 and positions.size(0) in (1, batch)
+           and positions.size(1) == length and positions.size(2) == axes,
+           "positions must be [L] or [1 or B, L], with a last dimension of one value per axis "
+           "when axis_pairs is given")
+    counts = None if axis_pairs is None else (ctypes.c_int32 * axes)(*axis_pairs)
+    return positions.contiguous(), inv_freq.to(torch.float64).contiguous(), axes, counts
+
+
+def turing_rope(query, key, positions, inv_freq, tensor_layout="HND", split_half=False,
+                axis_pairs=None, scale=1.0, inverse=False):
+    """Rotary positions on the first 2 * len(inv_freq) channels of each head of
+    query and (unless None) key, in one launch.  Returns new contiguous tensors
+    (key's is None when key is).  Not a reference binding."""
+    _check(tensor_layout in ("HND", "NHD"), f"Unsupported tensor_layout: {tensor_layout}")
+    layout = _lib.TB_LAYOUT_NHD if tensor_layout == "NHD" else _lib.TB_LAYOUT_HND
+    head_axis, seq_axis = (1, 2) if layout == _lib.TB_LAYOUT_HND else (2, 1)
+    tensors = [query] if key is None else [query, key]
+    for t in tensors:
+        _check(t.is_cuda and t.dim() == 4, "rotary input must be a 4D CUDA tensor")
+        _check_float_like(t, "rotary input")
+        _check(t.device == query.device and t.dtype == query.dtype
+               and t.size(0) == query.size(0) and t.size(seq_axis) == query.size(seq_axis)
+               and t.size(3) == query.size(3),
+               "query and key must share device, dtype, batch, length, and head dimension")
+    tensors = [t if t.stride(3) == 1 or t.size(3) == 1 else t.contiguous() for t in tensors]
+    batch, length, head_dim = query.size(0), query.size(seq_axis), query.size(3)
+    rot_dim = 2 * inv_freq.numel()
+    _check(rot_dim <= head_dim, "rot_dim must be even and within the head dimension")
+    _check(math.isfinite(scale), "scale must be finite")
+    positions, inv_freq, axes, counts = _rope_positions(positions, inv_freq, axis_pairs, batch,
+                                                        length, query.device)
+    with torch.cuda.device(query.device):
+        _require_blackwell(query.device, "rotary positions")
+        outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in tensors]
+        # A tensor without elements (no tokens, or a key without heads) takes no part.
+        live = [(t, o) for t, o in zip(tensors, outs) if t.numel() > 0]
+        if live:
+            (t0, o0), (t1, o1) = live[0], live[1] if len(live) > 1 else (None, None)
+            strides = (ctypes.c_int64 * 12)(
+                *layout_strides(t0, layout), *(layout_strides(t1, layout) if live[1:] else (0,) * 3),
+                *layout_strides(o0, layout), *(layout_strides(o1, layout) if live[1:] else (0,) * 3))
+            call("tb_rope", ptr(t0), ptr(t1), ptr(o0), ptr(o1), ptr(positions),
+                 POSITION_TYPES[positions.dtype], positions.size(0), ptr(inv_freq), counts, axes,
+                 batch, t0.size(head_axis), t1.size(head_axis) if live[1:] else 0, length,
+                 head_dim, rot_dim, strides, int(bool(split_half)), int(bool(inverse)),
+                 float_dtype_code(query), float(scale), stream_of(query))
+    return (outs[0], None) if key is None else (outs[0], outs[1])
+
+
+def turing_rope_freqs(positions, inv_freq, axis_pairs=None, scale=1.0, dtype=torch.bfloat16):
+    """The rotations as matrices scale * [[cos, -sin], [sin, cos]], [1 or B, L, 1,
+    len(inv_freq), 2, 2]: the freqs operand of the fused Q/K prologue.  Not a
+    reference binding."""
+    _check(positions.is_cuda, "rotary positions and frequencies must use the input's CUDA device")
+    lead = positions.dim() - (0 if axis_pairs is None else 1)
+    _check(lead in (1, 2), "positions must be [L] or [1 or B, L], with a last dimension of one "
+                           "value per axis when axis_pairs is given")
+    batch, length = (1, positions.size(0)) if lead == 1 else positions.shape[:2]
+    _check(dtype in (torch.float16, torch.bfloat16, torch.float32),
+           "rotary matrices must be float16, bfloat16, or float32")
+    _check(math.isfinite(scale), "scale must be finite")
+    dev = positions.device
+    positions, inv_freq, axes, counts = _rope_positions(positions, inv_freq, axis_pairs, batch,
+                                                        length, dev)
+    with torch.cuda.device(dev):
+        _require_blackwell(dev, "rotary positions")
+        out = torch.empty((batch, length, 1, inv_freq.numel(), 2, 2), dtype=dtype, device=dev)
+        if out.numel() > 0:
+            call("tb_rope_freqs", ptr(positions), POSITION_TYPES[positions.dtype],
+                 positions.size(0), ptr(inv_freq), counts, axes, ptr(out), batch, length,
+                 inv_freq.numel(), float_dtype_code(out), float(scale), stream_of(positions))
     return out

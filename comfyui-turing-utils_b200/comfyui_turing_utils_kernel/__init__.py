@@ -18,6 +18,10 @@ from .ops import (
     turing_layer_norm_adaln,
     turing_int8_gemm_s32,
     turing_int8_linear,
+    turing_rope,
+    turing_rope_freqs,
+    turing_rope_inv_freq,
+    turing_rope_qk,
     turing_swiglu_int4_convrot_quantize,
     turing_segmented_rms_adaln,
     turing_swiglu_int8_convrot_quantize,
@@ -44,5 +48,9 @@ __all__ = [
     "turing_w4a8_linear",
     "turing_segmented_rms_adaln",
     "turing_layer_norm_adaln",
+    "turing_rope",
+    "turing_rope_freqs",
+    "turing_rope_inv_freq",
+    "turing_rope_qk",
     "turing_sage",
 ]

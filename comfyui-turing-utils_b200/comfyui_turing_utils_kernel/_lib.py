@@ -26,10 +26,13 @@ TB_DTYPE_F16 = 1
 TB_DTYPE_F32 = 2
 TB_LAYOUT_NHD = 0
 TB_LAYOUT_HND = 1
+# Element types of rotary positions (TB_POS_*).
+POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2, torch.float64: 3}
 
 _p = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
+_f64 = ctypes.c_double
 
 # name -> argtypes (all entry points return int).
 SIGNATURES: dict[str, list] = {
@@ -77,6 +80,9 @@ SIGNATURES: dict[str, list] = {
     "tb_quantize_v_int8": [_p, _int, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p, _p],
     "tb_w8a8_attn": [_p, _p, _p, _p, _p, _int, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _p,
                      _int, ctypes.c_float, _p],
+    "tb_rope": [_p, _p, _p, _p, _p, _int, _i64, _p, _p, _int, _i64, _i64, _i64, _i64, _i64, _i64,
+                _p, _int, _int, _int, _f64, _p],
+    "tb_rope_freqs": [_p, _int, _i64, _p, _p, _int, _p, _i64, _i64, _i64, _int, _f64, _p],
 }
 
 _lock = threading.Lock()
@@ -131,6 +137,16 @@ def device_error() -> int:
 
 def ptr(t: torch.Tensor | None):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
+
+
+def layout_strides(t: torch.Tensor, layout: int) -> tuple[int, int, int]:
+    """(batch, head, token) element strides of a 4-D tensor in layout NHD or HND.
+    A dimension of one element gets the stride that a contiguous tensor of this
+    layout has: its own may be any number."""
+    _, n1, n2, d = t.shape
+    natural = (n1 * n2 * d, n2 * d, d)
+    s = [t.stride(i) if t.size(i) != 1 else natural[i] for i in range(3)]
+    return (s[0], s[2], s[1]) if layout == TB_LAYOUT_NHD else (s[0], s[1], s[2])
 
 
 def stream_of(t: torch.Tensor):

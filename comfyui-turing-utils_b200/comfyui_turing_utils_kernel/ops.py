@@ -8,6 +8,8 @@ kernels of libturing_b200.so through ``_C``.
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import _C
@@ -322,3 +324,214 @@ def turing_layer_norm_adaln(
 @turing_layer_norm_adaln.register_fake
 def _layer_norm_adaln_fake(x, scale, shift, epsilon=1.0e-5):
     return torch.empty_like(x)
+
+
+# ----------------------------------------------------------- rotary positions
+
+def turing_rope_inv_freq(
+    rot_dim: int,
+    theta: float = 10000.0,
+    *,
+    axis_pairs: list[int] | None = None,
+    scaling: str = "none",
+    factor: float = 1.0,
+    original_length: int = 0,
+    beta_fast: float = 32.0,
+    beta_slow: float = 1.0,
+    device: torch.device | str | None = None,
+) -> tuple[torch.Tensor, float]:
+    """Rotary frequencies, fp64 [rot_dim / 2], and the scale to rotate with.
+
+    Pair i of an axis of n pairs (one axis without axis_pairs) turns by
+    theta^(-i / n) per position.  For contexts `factor` times as long as trained:
+      "linear"  divides every frequency by factor;
+      "ntk"     raises theta to theta * factor^(n / (n - 1)), which keeps the
+                fastest frequency and divides the slowest by factor;
+      "yarn"    divides the frequencies that turn less than beta_slow times in
+                original_length tokens, keeps those above beta_fast turns, blends
+                linearly in the pair index between, and scales by
+                0.1 ln(factor) + 1.
+    Otherwise the scale is 1.
+    """
+    if rot_dim <= 0 or rot_dim % 2:
+        raise ValueError("rot_dim must be positive and even")
+    if not (math.isfinite(theta) and theta > 1.0):
+        raise ValueError("theta must be finite and larger than 1")
+    if scaling not in {"none", "linear", "ntk", "yarn"}:
+        raise ValueError(f"Unknown rotary scaling: {scaling}")
+    if not (math.isfinite(factor) and factor >= 1.0):
+        raise ValueError("factor must be finite and at least 1")
+    if scaling == "yarn" and (original_length <= 0 or not beta_fast > beta_slow > 0.0):
+        raise ValueError("yarn needs original_length > 0 and beta_fast > beta_slow > 0")
+    parts = [rot_dim // 2] if axis_pairs is None else [int(n) for n in axis_pairs]
+    if min(parts, default=-1) < 0 or sum(parts) != rot_dim // 2:
+        raise ValueError("axis_pairs must add up to rot_dim / 2")
+    freqs = []
+    for n in parts:
+        i = torch.arange(n, dtype=torch.float64)
+        base = theta * factor ** (n / (n - 1)) if scaling == "ntk" and n > 1 else theta
+        f = base ** (-i / max(n, 1))
+        if scaling == "linear":
+            f = f / factor
+        elif scaling == "yarn":
+            def pair_of(turns):  # the pair that turns this often in original_length
+                return n * math.log(original_length / (turns * 2.0 * math.pi)) / math.log(theta)
+            low = max(math.floor(pair_of(beta_fast)), 0)
+            high = min(math.ceil(pair_of(beta_slow)), n - 1)
+            slow = ((i - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
+            f = f * (1.0 - slow) + f / factor * slow
+        freqs.append(f)
+    scale = 0.1 * math.log(factor) + 1.0 if scaling == "yarn" else 1.0
+    return torch.cat(freqs).to(device), scale
+
+
+@torch.library.custom_op("turing_utils::rope", mutates_args=())
+def _rope_op(
+    x: torch.Tensor,
+    positions: torch.Tensor,
+    inv_freq: torch.Tensor,
+    tensor_layout: str = "HND",
+    split_half: bool = False,
+    axis_pairs: list[int] | None = None,
+    scale: float = 1.0,
+    inverse: bool = False,
+) -> torch.Tensor:
+    _require_cuda(x, "Rotary positions")
+    return _C.turing_rope(x, None, positions, inv_freq, tensor_layout, split_half, axis_pairs,
+                          scale, inverse)[0]
+
+
+@_rope_op.register_fake
+def _rope_fake(x, positions, inv_freq, tensor_layout="HND", split_half=False, axis_pairs=None,
+               scale=1.0, inverse=False):
+    return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
+@torch.library.custom_op("turing_utils::rope_qk", mutates_args=())
+def _rope_qk_op(
+    query: torch.Tensor,
+    key: torch.Tensor,
+    positions: torch.Tensor,
+    inv_freq: torch.Tensor,
+    tensor_layout: str = "HND",
+    split_half: bool = False,
+    axis_pairs: list[int] | None = None,
+    scale: float = 1.0,
+    inverse: bool = False,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    _require_cuda(query, "Rotary positions")
+    return _C.turing_rope(query, key, positions, inv_freq, tensor_layout, split_half, axis_pairs,
+                          scale, inverse)
+
+
+@_rope_qk_op.register_fake
+def _rope_qk_fake(query, key, positions, inv_freq, tensor_layout="HND", split_half=False,
+                  axis_pairs=None, scale=1.0, inverse=False):
+    return (torch.empty(query.shape, dtype=query.dtype, device=query.device),
+            torch.empty(key.shape, dtype=key.dtype, device=key.device))
+
+
+def _rope_setup(ctx, inputs, output):
+    tensors = len(inputs) - 7
+    ctx.save_for_backward(*inputs[tensors:tensors + 2])
+    ctx.options = inputs[tensors + 2:]
+
+
+def _rope_grad_args(ctx):
+    layout, split_half, axis_pairs, scale, inverse = ctx.options
+    return (*ctx.saved_tensors, layout, split_half, axis_pairs, scale, not inverse)
+
+
+def _rope_backward(ctx, grad):
+    return (_rope_op(grad, *_rope_grad_args(ctx)), *(None,) * 7)
+
+
+def _rope_qk_backward(ctx, grad_query, grad_key):
+    args = _rope_grad_args(ctx)
+    need_q = ctx.needs_input_grad[0] and grad_query is not None
+    need_k = ctx.needs_input_grad[1] and grad_key is not None
+    if need_q and need_k:
+        return (*_rope_qk_op(grad_query, grad_key, *args), *(None,) * 7)
+    return (_rope_op(grad_query, *args) if need_q else None,
+            _rope_op(grad_key, *args) if need_k else None, *(None,) * 7)
+
+
+_rope_op.register_autograd(_rope_backward, setup_context=_rope_setup)
+_rope_qk_op.register_autograd(_rope_qk_backward, setup_context=_rope_setup)
+
+
+def turing_rope(
+    x: torch.Tensor,
+    positions: torch.Tensor,
+    inv_freq: torch.Tensor,
+    *,
+    tensor_layout: str = "HND",
+    split_half: bool = False,
+    axis_pairs: list[int] | None = None,
+    scale: float = 1.0,
+    inverse: bool = False,
+) -> torch.Tensor:
+    """Rotary positions on x [B, H, L, D] (HND) or [B, L, H, D] (NHD), float16,
+    bfloat16 or float32, differentiable in x.
+
+    The first 2 * len(inv_freq) channels of each head turn; the others are
+    copied.  Pair p, channels (2p, 2p + 1) or with split_half (p, p + pairs),
+    turns by position * inv_freq[p] (the angle is taken in fp64) and is
+    multiplied by scale.  positions: int32, int64, float32 or float64, [L] or
+    [1 or B, L]; with axis_pairs (pairs of each of 1 to 4 axes) [L, axes] or
+    [1 or B, L, axes].  inverse turns the other way.
+    """
+    return _rope_op(x, positions, inv_freq, tensor_layout, split_half, axis_pairs, float(scale),
+                    inverse)
+
+
+def turing_rope_qk(
+    query: torch.Tensor,
+    key: torch.Tensor,
+    positions: torch.Tensor,
+    inv_freq: torch.Tensor,
+    *,
+    tensor_layout: str = "HND",
+    split_half: bool = False,
+    axis_pairs: list[int] | None = None,
+    scale: float = 1.0,
+    inverse: bool = False,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """turing_rope of query and key (same batch, length and head dimension, any
+    head counts) in one launch, differentiable in both."""
+    return _rope_qk_op(query, key, positions, inv_freq, tensor_layout, split_half, axis_pairs,
+                       float(scale), inverse)
+
+
+@torch.library.custom_op("turing_utils::rope_freqs", mutates_args=())
+def _rope_freqs_op(
+    positions: torch.Tensor,
+    inv_freq: torch.Tensor,
+    axis_pairs: list[int] | None,
+    scale: float,
+    dtype: torch.dtype,
+) -> torch.Tensor:
+    _require_cuda(positions, "Rotary positions")
+    return _C.turing_rope_freqs(positions, inv_freq, axis_pairs, scale, dtype)
+
+
+@_rope_freqs_op.register_fake
+def _rope_freqs_fake(positions, inv_freq, axis_pairs, scale, dtype):
+    lead = positions.shape if axis_pairs is None else positions.shape[:-1]
+    batch, length = (1, lead[0]) if len(lead) == 1 else lead
+    return torch.empty((batch, length, 1, inv_freq.size(0), 2, 2), dtype=dtype,
+                       device=positions.device)
+
+
+def turing_rope_freqs(
+    positions: torch.Tensor,
+    inv_freq: torch.Tensor,
+    *,
+    axis_pairs: list[int] | None = None,
+    scale: float = 1.0,
+    dtype: torch.dtype = torch.bfloat16,
+) -> torch.Tensor:
+    """The rotations of turing_rope as matrices scale * [[cos, -sin], [sin, cos]],
+    [1 or B, L, 1, len(inv_freq), 2, 2]: the freqs argument of
+    turing_sage.prequantize_rms_rope_qk."""
+    return _rope_freqs_op(positions, inv_freq, axis_pairs, float(scale), dtype)

@@ -43,6 +43,12 @@ extern "C" {
 #define TB_LAYOUT_NHD 0
 #define TB_LAYOUT_HND 1
 
+/* Element types of rotary positions. */
+#define TB_POS_I32 0
+#define TB_POS_I64 1
+#define TB_POS_F32 2
+#define TB_POS_F64 3
+
 typedef void *tb_stream_t;
 
 /* Exported symbols (the library is built with hidden default visibility). */
@@ -411,6 +417,38 @@ TB_API int tb_w8a8_attn(const int8_t *q, const int8_t *k, const void *v_codes,
                         const float *k_scale, int64_t B, int64_t Hq, int64_t Hk, int64_t Lq,
                         int64_t Lk, int64_t D, const int64_t *strides, int is_causal,
                         float sm_scale, tb_stream_t stream);
+
+/* ---------------------------------------------------- rotary positions -- */
+
+/* Rotary positions on the first rot_dim channels of each head of Q and
+ * (optionally: key, key_out NULL and key_heads 0 without) K in one launch; the
+ * other channels are copied.  Pair p, channels (2p, 2p + 1) or with split_half
+ * (p, p + rot_dim / 2), turns by position * inv_freq[p] (fp64 [rot_dim / 2]),
+ * by the negative angle when inverse != 0 (the gradient), and is multiplied by
+ * scale.  positions: contiguous [position_batches, length, axes] of type
+ * TB_POS_*, position_batches 1 (shared) or batch; axis_pairs (host, int32
+ * [axes], or NULL for one axis) counts the pairs that turn with each axis.
+ * strides (elements, 12 values): query (b, h, l), key (b, h, l), query_out
+ * (b, h, l), key_out (b, h, l); the last dimension is contiguous.  Any
+ * alignment; 16-byte aligned rows take the vector kernel.  An output may be
+ * its input.  dtype BF16 / F16 / F32.  No counterpart in the reference (its
+ * rotation runs inside the fused Q/K prologue from ready-made matrices,
+ * kernel/csrc/turing/sage/qk_preprocess.cu:151-201). */
+TB_API int tb_rope(const void *query, const void *key, void *query_out, void *key_out,
+                   const void *positions, int position_type, int64_t position_batches,
+                   const double *inv_freq, const int32_t *axis_pairs, int axes, int64_t batch,
+                   int64_t query_heads, int64_t key_heads, int64_t length, int64_t head_dim,
+                   int64_t rot_dim, const int64_t *strides, int split_half, int inverse,
+                   int dtype, double scale, tb_stream_t stream);
+
+/* The rotations as 2x2 matrices scale * [[cos, -sin], [sin, cos]]: output
+ * [batch, length, pairs, 2, 2] contiguous, 16-byte aligned, the freqs operand
+ * of tb_quant_qk_rms_rope_int8 and tb_qk_rms_rope_apply.  Other arguments as
+ * for tb_rope.  No counterpart in the reference. */
+TB_API int tb_rope_freqs(const void *positions, int position_type, int64_t position_batches,
+                         const double *inv_freq, const int32_t *axis_pairs, int axes,
+                         void *output, int64_t batch, int64_t length, int64_t pairs, int dtype,
+                         double scale, tb_stream_t stream);
 
 #ifdef __cplusplus
 }
