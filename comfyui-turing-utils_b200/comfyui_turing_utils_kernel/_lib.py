@@ -83,6 +83,12 @@ SIGNATURES: dict[str, list] = {
     "tb_rope": [_p, _p, _p, _p, _p, _int, _i64, _p, _p, _int, _i64, _i64, _i64, _i64, _i64, _i64,
                 _p, _int, _int, _int, _f64, _p],
     "tb_rope_freqs": [_p, _int, _i64, _p, _p, _int, _p, _i64, _i64, _i64, _int, _f64, _p],
+    "tb_select_key_blocks_workspace": [_i64, _i64, _i64, _i64, _i64, _i64, _p],
+    "tb_select_key_blocks": [_p, _p, _p, _p, _p, _p, _i64, _p, _p, _i64, _i64, _i64, _i64, _i64,
+                             _i64, _i64, _i64, _p, _p],
+    "tb_sparse_attn_workspace": [_i64, _i64, _i64, _i64, _p],
+    "tb_sparse_attn": [_p, _p, _p, _int, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64,
+                       _i64, _i64, _i64, _p, ctypes.c_float, _p],
 }
 
 _lock = threading.Lock()

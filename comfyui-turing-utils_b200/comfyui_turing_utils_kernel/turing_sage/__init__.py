@@ -129,6 +129,47 @@ def w8a8attn_compiled(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
                           int(key_tile_tokens), bool(rotate_qk), bool(stabilize_k))
 
 
+def sparse_sageattn(*args, **kwargs):
+    """Block-sparse Sage INT8 attention over the best-scoring key blocks of each
+    query block (no counterpart in the reference: its Sol routes are not built)."""
+    from .sparse import sparse_sageattn as _impl
+
+    return _impl(*args, **kwargs)
+
+
+def sparse_sageattn_compiled(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
+                             keep: int, *, tensor_layout: str = "HND",
+                             sm_scale: float | None = None, smooth_k: bool = False,
+                             key_lengths: torch.Tensor | None = None,
+                             block_policy: torch.Tensor | None = None) -> torch.Tensor:
+    """torch.compile leaf of sparse_sageattn."""
+    from .custom_ops import sparse_sage_attention
+
+    return sparse_sage_attention(query, key, value, int(keep), tensor_layout,
+                                 -1.0 if sm_scale is None else float(sm_scale), bool(smooth_k),
+                                 key_lengths, block_policy)
+
+
+def sparse_sageattn_from_prequantized(*args, **kwargs):
+    from .sparse import sparse_sageattn_from_prequantized as _impl
+
+    return _impl(*args, **kwargs)
+
+
+def sparse_sageattn_prequantized(*args, **kwargs):
+    """Sage INT8 attention over given lists of key blocks."""
+    from .sparse import sparse_sageattn_prequantized as _impl
+
+    return _impl(*args, **kwargs)
+
+
+def select_key_blocks(*args, **kwargs):
+    """The key blocks that score highest for each query block."""
+    from .sparse import select_key_blocks as _impl
+
+    return _impl(*args, **kwargs)
+
+
 def prequantize_sol_sageattn(*args, **kwargs):
     from .core import prequantize_sol_sageattn as _impl
 
@@ -257,7 +298,9 @@ __all__ = ["available", "fused_qk_preprocessing_available", "overlap_accumulate_
            "prequantize_rms_rope_qk", "prequantize_sageattn", "prequantize_sageattn_from_qk",
            "prequantize_sol_sageattn", "prequantize_sol_sageattn_from_qk",
            "quantize_key_per_block", "rms_rope_per_warp_int8", "quantize_query_per_warp",
-           "sageattn", "sageattn_compiled", "sageattn_from_prequantized", "sla_available",
+           "sageattn", "sageattn_compiled", "sageattn_from_prequantized", "select_key_blocks",
+           "sla_available", "sparse_sageattn", "sparse_sageattn_compiled",
+           "sparse_sageattn_from_prequantized", "sparse_sageattn_prequantized",
            "sol_sparse_sageattn_from_prequantized", "sparse_available",
            "split_prequantization_available", "w8a8_available", "w8a8_varlen_available",
            "w8a8attn", "w8a8attn_compiled"]

@@ -1,7 +1,9 @@
 """``turing_utils::sage_attention`` (turing_sage/custom_ops.py:137-167),
 ``turing_utils::w8a8_attention`` (custom_ops.py:170-210) and
 ``turing_utils::qk_rms_rope_int8`` (custom_ops.py:63-130) custom ops: same
-schemas and fake implementations, backed by the sm_100a kernels."""
+schemas and fake implementations, backed by the sm_100a kernels.
+``turing_utils::sparse_sage_attention`` (no counterpart in the reference) is the
+block-sparse form."""
 from __future__ import annotations
 
 import torch
@@ -71,3 +73,22 @@ def w8a8_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
 def _w8a8_attention_fake(query, key, value, tensor_layout, is_causal, sm_scale, key_tile_tokens,
                          rotate_qk, stabilize_k):
     return torch.empty_like(query)
+
+
+@torch.library.custom_op("turing_utils::sparse_sage_attention", mutates_args=())
+def sparse_sage_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, keep: int,
+                          tensor_layout: str, sm_scale: float, smooth_k: bool,
+                          key_lengths: torch.Tensor | None,
+                          block_policy: torch.Tensor | None) -> torch.Tensor:
+    from .sparse import sparse_sageattn
+
+    # A custom op's result is contiguous: heads below 128 come back as a slice.
+    return sparse_sageattn(query, key, value, keep, tensor_layout=tensor_layout,
+                           sm_scale=sm_scale if sm_scale > 0.0 else None, smooth_k=smooth_k,
+                           key_lengths=key_lengths, block_policy=block_policy).contiguous()
+
+
+@sparse_sage_attention.register_fake
+def _sparse_sage_attention_fake(query, key, value, keep, tensor_layout, sm_scale, smooth_k,
+                                key_lengths, block_policy):
+    return torch.empty(query.shape, dtype=query.dtype, device=query.device)

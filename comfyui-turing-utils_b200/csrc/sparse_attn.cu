@@ -1,0 +1,636 @@
+// Block-sparse Sage INT8 attention for sm_100a (tcgen05 + TMA + TMEM).
+//
+// Each block of 128 query rows attends to the key blocks (64 keys, one k_scale
+// block) that its list names; with L the listed keys below key_lengths[b],
+//   S_int = Q8 . K8^T                      (exact INT32, tensor core kind::i8)
+//   s     = S_int * (sm_scale * log2 e * q_scale[row / 16] * k_scale[key / 64])
+//   p = 2^(s - m), d = sum_L p, O = sum_L p V, out = O / d, lse = ln sum_L e^..
+// with the running reference m of one pass over the list (moved, and O and d
+// rescaled, only when a row's max grows by more than 2^8 over it).  A row that
+// sees no key gives 0 and lse = -inf.  S, m, d and O are INT32 / fp32; p is
+// rounded to V's 16-bit type for the second contraction (half a step 2^-9 bf16,
+// 2^-12 fp16 relative, averaged over the keys: below the output's own
+// rounding), d sums the unrounded p.  s - m is one FMA of the exactly converted
+// score: no error that grows with the scales.
+//
+// Lists of neighbouring query blocks differ, so nothing is shared between query
+// tiles: a CTA takes one query block (128 rows x one head) and two CTAs share
+// an SM (113 KB of shared memory, 256 TMEM columns, 192 threads each), one's
+// barrier waits and tile ends filled by the other:
+//   warps 0-3  softmax, one query row per thread (TMEM lane quadrant = warp);
+//   warp 4     TMA producer: Q once, then K (8 KB) and V (16 KB) of the listed
+//              blocks into a 4-stage ring (128B swizzle);
+//   warp 5     MMA issuer: S = Q K_j^T into one of two S buffers, O += P V_j.
+// TMEM columns: O [0, 128), S(b) at 128 + 64 b; P(j) overwrites the first 32
+// columns of its S buffer.  While the softmax turns S(j) into P, the tensor
+// core computes S(j + 1).
+//
+// Few query blocks (single tokens): the list is split over CTAs, which write
+// unnormalized O, m and d; sparse_combine_kernel joins them.
+//
+// List entries that name no block with visible keys (negative, or at or past
+// the end) are skipped by every role alike: the producer and softmax warps walk
+// the list 32 entries at a time with a warp vote, and the count the prologue
+// takes bounds all loops.  A block named twice counts twice.
+#define TB_TRY_WAIT_NO_HINT 1
+#include <algorithm>
+#include <cmath>
+
+#include "attn_common.cuh"
+#include "tb_capi_internal.h"
+#include "tb_tu.cuh"
+
+namespace tb {
+namespace {
+
+constexpr int kRows = 128;   // query block
+constexpr int kKeys = 64;    // key block
+constexpr int kDim = 128;
+constexpr int kStages = 4;
+constexpr int kSoftmaxWarps = 4;
+constexpr int kProducerWarp = 4;
+constexpr int kMmaWarp = 5;
+constexpr int kThreads = 192;
+constexpr int kQBytes = kRows * kDim;
+constexpr int kKBytes = kKeys * kDim;
+constexpr int kVBytes = kKeys * kDim * 2;
+constexpr int kStageBytes = kKBytes + kVBytes;
+constexpr int kDataBytes = kQBytes + kStages * kStageBytes;
+constexpr uint32_t kTmemCols = 256;
+constexpr uint32_t kSBase = 128;
+constexpr int kCombineWarps = 4;
+
+struct SparseParams {
+  int Hq, Hk, Lq, Lk, groups;   // groups = Hq / Hk
+  int query_blocks, keep, splits, chunk;
+  int q_tiles_scale, k_tiles_scale;
+  const float* q_scale;
+  const float* k_scale;
+  const int32_t* lists;         // [B, Hq, query_blocks, keep]
+  const int32_t* key_lengths;   // [B] or null
+  void* out;
+  int64_t o_sb, o_sh, o_sl;
+  float* lse;                   // [B, Hq, Lq] natural logarithm, or null
+  float sm_scale_log2;
+  float* part_o;                // [B * Hq * Lq, splits, kDim] when splits > 1
+  float2* part_md;              // [B * Hq * Lq, splits] (m, d)
+};
+
+struct __align__(8) SparseBarriers {
+  uint64_t q_full;
+  uint64_t kv_full[kStages];
+  uint64_t kv_empty[kStages];
+  uint64_t s_full[2];   // S buffer b computed
+  uint64_t p_full[2];   // the 4 softmax warps stored P in buffer b
+  uint64_t o_done;      // after each of the last two PVs
+  uint64_t o_final;     // after the last PV
+  uint64_t drain;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+constexpr int kSmemBytes = kDataBytes + static_cast<int>(sizeof(SparseBarriers));
+static_assert(2 * (kSmemBytes + 1024) <= 228 * 1024, "two CTAs must fit one SM");
+
+// Walks the visible entries of a list slice, the warp together.
+struct ListCursor {
+  const int32_t* list;
+  int n, visible, base, value;
+  uint32_t mask;
+  __device__ __forceinline__ ListCursor(const int32_t* l, int count, int visible_blocks)
+      : list(l), n(count), visible(visible_blocks), base(-32), value(0), mask(0) {}
+  __device__ __forceinline__ int next() {
+    while (mask == 0 && base + 32 < n) {
+      base += 32;
+      const int i = base + static_cast<int>(lane_id());
+      value = i < n ? __ldg(list + i) : -1;
+      mask = __ballot_sync(0xffffffffu, static_cast<uint32_t>(value) <
+                                            static_cast<uint32_t>(visible));
+    }
+    const int at = mask != 0 ? __ffs(static_cast<int>(mask)) - 1 : 0;
+    mask &= mask - 1;
+    const int v = __shfl_sync(0xffffffffu, value, at);
+    // Always a block of the tensor, whatever the list holds by now.
+    return static_cast<uint32_t>(v) < static_cast<uint32_t>(visible) ? v : 0;
+  }
+};
+
+// p = 2^(s c - m) of the 64 scores of a block, in place as packed pairs of
+// V's type; `sum2` gathers the unrounded p.  Returns the integer row max where
+// TRACK_MAX.  MASKED zeroes keys >= valid.  WAIT_HI: columns 32..63 are still
+// loading.
+template <typename TV, bool TRACK_MAX, bool MASKED, bool WAIT_HI>
+__device__ __forceinline__ int exp_scores(uint32_t (&v)[kKeys], uint64_t c2, uint64_t nm2,
+                                          int valid, uint64_t (&sum2)[2]) {
+  int m[4] = {INT32_MIN, INT32_MIN, INT32_MIN, INT32_MIN};
+#pragma unroll
+  for (int i = 0; i < kKeys / 2; ++i) {
+    if (WAIT_HI && i == kKeys / 4) tmem_wait_ld_regs(*reinterpret_cast<uint32_t(*)[32]>(v + 32));
+    if (TRACK_MAX)
+      m[i & 3] =
+          __vimax3_s32(m[i & 3], static_cast<int>(v[2 * i]), static_cast<int>(v[2 * i + 1]));
+    uint64_t p2 = ex2_pair(f2_fma(score_pair_f32(v[2 * i], v[2 * i + 1]), c2, nm2));
+    if (MASKED)
+      p2 = f2_pack(2 * i < valid ? f2_lo(p2) : 0.0f, 2 * i + 1 < valid ? f2_hi(p2) : 0.0f);
+    sum2[i & 1] = f2_add(sum2[i & 1], p2);
+    v[i] = pack_pair<TV>(p2);
+  }
+  return max(max(m[0], m[1]), max(m[2], m[3]));
+}
+
+template <typename TV>
+__global__ void __launch_bounds__(kThreads, 2)
+    sparse_attn_kernel(const __grid_constant__ CUtensorMap tm_q,
+                       const __grid_constant__ CUtensorMap tm_k,
+                       const __grid_constant__ CUtensorMap tm_v, const SparseParams p) {
+  extern __shared__ __align__(1024) unsigned char smem[];
+  unsigned char* kv_smem = smem + kQBytes;
+  SparseBarriers* bar = reinterpret_cast<SparseBarriers*>(smem + kDataBytes);
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+
+  const int split = blockIdx.x % p.splits;
+  const int tile = blockIdx.x / p.splits;
+  const int qb = tile % p.query_blocks;
+  const int bh = tile / p.query_blocks;
+  const int b = bh / p.Hq;
+  const int h = bh % p.Hq;
+  const int hk = h / p.groups;
+  const int q0 = qb * kRows;
+  const int key_len = p.key_lengths != nullptr ? max(0, min(__ldg(p.key_lengths + b), p.Lk)) : p.Lk;
+  const int visible = (key_len + kKeys - 1) / kKeys;
+  const int32_t* list = p.lists + (static_cast<int64_t>(bh) * p.query_blocks + qb) * p.keep +
+                        static_cast<int64_t>(split) * p.chunk;
+  const int n_list = min(p.chunk, p.keep - split * p.chunk);
+
+  if (threadIdx.x == 0) {
+    mbar_init(&bar->q_full, 1);
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&bar->kv_full[s], 1);
+      mbar_init(&bar->kv_empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar->s_full[i], 1);
+      mbar_init(&bar->p_full[i], kSoftmaxWarps);
+    }
+    mbar_init(&bar->o_done, 1);
+    mbar_init(&bar->o_final, 1);
+    mbar_init(&bar->drain, 1);
+    bar->abort_flag = 0;
+    fence_barrier_init();
+    // The swizzle atoms need 1024-byte aligned tiles (the array asks for it).
+    if ((smem_u32(smem) & 1023u) != 0) {
+      record_device_error(kDevBadLaunch);
+      bar->abort_flag = 1;
+    }
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(&bar->tmem_base, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  int n_kv = 0;
+  for (int i = 0; i < n_list; i += kThreads) {
+    const int at = i + static_cast<int>(threadIdx.x);
+    n_kv += __syncthreads_count(at < n_list && static_cast<uint32_t>(__ldg(list + at)) <
+                                                   static_cast<uint32_t>(visible));
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bar->tmem_base;
+  volatile int* abort_flag = &bar->abort_flag;
+  if (*abort_flag) n_kv = 0;
+
+  if (warp == kProducerWarp) {
+    // ------------------------------------------------------------ producer
+    if (n_kv > 0) {
+      if (lane == 0) {
+        tma_prefetch_desc(&tm_k);
+        tma_prefetch_desc(&tm_v);
+        mbar_arrive_expect_tx(&bar->q_full, kQBytes);
+        tma_load_4d(smem, &tm_q, &bar->q_full, 0, q0, h, b);
+      }
+      ListCursor cur(list, n_list, visible);
+      int stage = 0, issued = 0;
+      uint32_t phase = 0;
+      for (int j = 0; j < n_kv; ++j) {
+        const int blk = cur.next();
+        bool ok = true;
+        if (lane == 0) {
+          ok = mbar_wait(&bar->kv_empty[stage], phase ^ 1u, abort_flag, kDevWaitTimeoutProducer);
+          if (ok) {
+            unsigned char* k_dst = kv_smem + stage * kStageBytes;
+            unsigned char* v_dst = k_dst + kKBytes;
+            mbar_arrive_expect_tx(&bar->kv_full[stage], kStageBytes);
+            tma_load_4d(k_dst, &tm_k, &bar->kv_full[stage], 0, blk * kKeys, hk, b);
+#pragma unroll
+            for (int dh = 0; dh < kDim / 64; ++dh)
+              tma_load_4d(v_dst + dh * (kKeys * 128), &tm_v, &bar->kv_full[stage], dh * 64,
+                          blk * kKeys, hk, b);
+          }
+        }
+        if (!__shfl_sync(0xffffffffu, static_cast<int>(ok), 0)) break;
+        ++issued;
+        if (++stage == kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (lane == 0) {
+        // Every copy issued by this CTA lands before it exits.
+        drain_wait(&bar->q_full, 0);
+        for (int i = min(issued, kStages); i > 0; --i) {
+          if (--stage < 0) {
+            stage = kStages - 1;
+            phase ^= 1u;
+          }
+          drain_wait(&bar->kv_full[stage], phase);
+        }
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0 && n_kv > 0) {
+      constexpr uint32_t idesc_qk = idesc_i8(kRows, kKeys);
+      constexpr uint32_t idesc_pv = idesc_f16(
+          kRows, kDim, std::is_same<TV, __nv_bfloat16>::value, /*b_mn_major=*/true);
+      const uint32_t kv_addr = smem_u32(kv_smem);
+      const uint64_t q_desc = umma_desc_sw128(smem_u32(smem));
+      auto issue_s = [&](int j) {
+        const uint32_t d_tmem = tmem + kSBase + static_cast<uint32_t>(j & 1) * kKeys;
+        const uint64_t bk = umma_desc_sw128(kv_addr + (j % kStages) * kStageBytes);
+#pragma unroll
+        for (int kk = 0; kk < kDim / 32; ++kk)
+          mma_i8_ss(d_tmem, q_desc + 2u * kk, bk + 2u * kk, idesc_qk, kk > 0 ? 1u : 0u);
+      };
+      auto wait_kv = [&](int j) {
+        return mbar_wait(&bar->kv_full[j % kStages], static_cast<uint32_t>(j / kStages) & 1u,
+                         abort_flag, kDevWaitTimeoutMma);
+      };
+      bool ok = mbar_wait(&bar->q_full, 0, abort_flag, kDevWaitTimeoutMma);
+      for (int j = 0; j < 2 && j < n_kv && ok; ++j) {
+        ok = wait_kv(j);
+        if (ok) {
+          tc_fence_after();
+          issue_s(j);
+          mma_commit(&bar->s_full[j & 1]);
+        }
+      }
+      // Both waits of a block first, then PV(j) and S(j + 2) back to back, then
+      // the commits.  The s_full commit of S(j + 2) also says that PV(j) is
+      // done; o_done marks the last two PVs, which no S commit follows.
+      for (int j = 0; j < n_kv && ok; ++j) {
+        const bool next_s = j + 2 < n_kv;
+        ok = mbar_wait(&bar->p_full[j & 1], static_cast<uint32_t>(j >> 1) & 1u, abort_flag,
+                       kDevWaitTimeoutMma) &&
+             (!next_s || wait_kv(j + 2));
+        if (!ok) break;
+        tc_fence_after();
+        const int stage = j % kStages;
+        const uint32_t v_addr = kv_addr + stage * kStageBytes + kKBytes;
+        const uint32_t p_tmem = tmem + kSBase + static_cast<uint32_t>(j & 1) * kKeys;
+#pragma unroll
+        for (int kk = 0; kk < kKeys / 16; ++kk) {
+          const uint64_t bv = umma_desc_sw128_mn(v_addr + kk * 2048, kKeys * 128, 1024);
+          mma_f16_ts(tmem, p_tmem + static_cast<uint32_t>(kk * 8), bv, idesc_pv,
+                     (j > 0 || kk > 0) ? 1u : 0u);
+        }
+        if (next_s) {
+          issue_s(j + 2);
+          mma_commit(&bar->s_full[j & 1]);
+        } else {
+          mma_commit(&bar->o_done);
+        }
+        mma_commit(&bar->kv_empty[stage]);
+        if (j + 1 == n_kv) mma_commit(&bar->o_final);
+      }
+      mma_commit(&bar->drain);
+      drain_wait(&bar->drain, 0);
+    }
+  } else {
+    // ------------------------------------------------------------ softmax
+    const int row = q0 + warp * 32 + lane;
+    const uint32_t lane_off = static_cast<uint32_t>(warp * 32) << 16;
+    const uint32_t s_tmem0 = tmem + lane_off + kSBase;
+    const uint32_t o_tmem = tmem + lane_off;
+    const float* ks_row = p.k_scale + static_cast<int64_t>(b * p.Hk + hk) * p.k_tiles_scale;
+    const float cq = row < p.Lq ? p.sm_scale_log2 * __ldg(p.q_scale + static_cast<int64_t>(bh) *
+                                                              p.q_tiles_scale + row / 16)
+                                : 0.0f;
+    float m_ref = -INFINITY;  // exponent reference point
+    float dsum = 0.0f;
+    bool ok = n_kv > 0;
+    ListCursor cur(list, n_list, visible);
+    int blk_next = ok ? cur.next() : 0;
+    float ks = ok ? __ldg(ks_row + blk_next) : 0.0f;
+    // tcgen05.ld / st are warp-collective: every branch around one is taken by
+    // a warp vote.
+    for (int j = 0; j < n_kv && ok; ++j) {
+      const int key0 = blk_next * kKeys;
+      const float c = cq * ks;
+      if (j + 1 < n_kv) {
+        blk_next = cur.next();
+        ks = __ldg(ks_row + blk_next);
+      }
+      ok = __all_sync(0xffffffffu,
+                      mbar_wait(&bar->s_full[j & 1], static_cast<uint32_t>(j >> 1) & 1u,
+                                abort_flag, kDevWaitTimeoutSoftmax));
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t s_tmem = s_tmem0 + static_cast<uint32_t>(j & 1) * kKeys;
+      const int valid = min(kKeys, key_len - key0);  // >= 1, the same for every row
+      uint32_t v[kKeys];
+      tmem_ld32(s_tmem, *reinterpret_cast<uint32_t(*)[32]>(v));
+      tmem_wait_ld_regs(*reinterpret_cast<uint32_t(*)[32]>(v));
+      tmem_ld32(s_tmem + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
+      const uint64_t c2 = f2_pack(c, c);
+      uint64_t sum2[2] = {0ull, 0ull};
+      bool done = false, need_rescale = false, hi_pending = true;
+      float f = 1.0f;
+      if (valid == kKeys && __all_sync(0xffffffffu, m_ref != -INFINITY)) {
+        // Usual case: the reference stands, so the exponentials need not wait
+        // for the row max; if it moved past, the block is read again below.
+        const int mx =
+            exp_scores<TV, true, false, true>(v, c2, f2_pack(-m_ref, -m_ref), valid, sum2);
+        hi_pending = false;
+        done = !__any_sync(0xffffffffu, i2f_exact(mx) * c > m_ref + 8.0f);
+        if (!done) {
+          sum2[0] = sum2[1] = 0ull;
+          tmem_ld32(s_tmem, *reinterpret_cast<uint32_t(*)[32]>(v));
+          tmem_ld32(s_tmem + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
+          tmem_wait_ld();
+        }
+      }
+      if (!done) {
+        if (hi_pending) tmem_wait_ld_regs(*reinterpret_cast<uint32_t(*)[32]>(v + 32));
+        int mx = INT32_MIN;
+#pragma unroll
+        for (int i = 0; i < kKeys; i += 2)
+          mx = __vimax3_s32(mx, i < valid ? static_cast<int>(v[i]) : INT32_MIN,
+                            i + 1 < valid ? static_cast<int>(v[i + 1]) : INT32_MIN);
+        const float m_blk = i2f_exact(mx) * c;
+        const bool move = m_blk > m_ref + 8.0f;
+        const bool rescale = move && m_ref != -INFINITY;
+        need_rescale = __any_sync(0xffffffffu, rescale);
+        f = rescale ? ex2(m_ref - m_blk) : 1.0f;
+        dsum *= f;
+        if (move) m_ref = m_blk;
+        const float nm = m_ref == -INFINITY ? 0.0f : -m_ref;
+        exp_scores<TV, false, true, false>(v, c2, f2_pack(nm, nm), valid, sum2);
+      }
+      tmem_st32(s_tmem, *reinterpret_cast<const uint32_t(*)[32]>(v));
+      const uint64_t s01 = f2_add(sum2[0], sum2[1]);
+      dsum += f2_lo(s01) + f2_hi(s01);
+      if (valid < kKeys && key_len < p.Lk) {
+        // V rows past key_lengths hold whatever the padding holds; a NaN there
+        // times p = 0 would still be NaN, so the rows are cleared.
+        ok = __all_sync(0xffffffffu,
+                        mbar_wait(&bar->kv_full[j % kStages],
+                                  static_cast<uint32_t>(j / kStages) & 1u, abort_flag,
+                                  kDevWaitTimeoutSoftmax));
+        if (!ok) break;
+        unsigned char* vt = kv_smem + (j % kStages) * kStageBytes + kKBytes;
+        for (int i = threadIdx.x; i < (kKeys - valid) * 16; i += kSoftmaxWarps * 32)
+          *reinterpret_cast<uint4*>(vt + (i & 8 ? kKeys * 128 : 0) + (valid + (i >> 4)) * 128 +
+                                    (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
+      }
+      if (need_rescale) {
+        // O holds PV(0 .. j-1) once the commit after PV(j - 1) arrived; PV(j)
+        // waits for this warp's p_full arrival below.
+        const bool waited =
+            j + 1 < n_kv
+                ? mbar_wait(&bar->s_full[(j + 1) & 1], static_cast<uint32_t>((j + 1) >> 1) & 1u,
+                            abort_flag, kDevWaitTimeoutSoftmax)
+                : mbar_wait(&bar->o_done, 0u, abort_flag, kDevWaitTimeoutSoftmax);
+        ok = __all_sync(0xffffffffu, waited);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll 1
+        for (int cc = 0; cc < kDim / 16; ++cc) {
+          uint32_t o[16];
+          tmem_ld16(o_tmem + cc * 16, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+          tmem_st16(o_tmem + cc * 16, o);
+        }
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar->p_full[j & 1]);
+    }
+    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&bar->o_final, 0u, abort_flag,
+                                                   kDevWaitTimeoutSoftmax));
+    if (ok || n_kv == 0) {
+      tc_fence_after();
+      const float inv = dsum > 0.0f ? 1.0f / dsum : (dsum == 0.0f ? 0.0f : dsum);
+      const int64_t flat = static_cast<int64_t>(bh) * p.Lq + row;
+      TV* orow = static_cast<TV*>(p.out) + b * p.o_sb + h * p.o_sh +
+                 static_cast<int64_t>(row) * p.o_sl;
+      float* prow = p.splits > 1 ? p.part_o + (flat * p.splits + split) * kDim : nullptr;
+#pragma unroll 1
+      for (int cc = 0; cc < kDim / 16; ++cc) {
+        uint32_t o[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] = 0u;
+        if (n_kv > 0) {
+          tmem_ld16(o_tmem + cc * 16, o);
+          tmem_wait_ld();
+        }
+        if (row >= p.Lq) continue;
+        if (prow != nullptr) {
+#pragma unroll
+          for (int i = 0; i < 16; i += 4)
+            *reinterpret_cast<uint4*>(prow + cc * 16 + i) =
+                make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        } else {
+          uint32_t w[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            w[i] = pack2<TV>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+          *reinterpret_cast<uint4*>(orow + cc * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+          *reinterpret_cast<uint4*>(orow + cc * 16 + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+        }
+      }
+      if (row < p.Lq) {
+        if (p.splits > 1) p.part_md[flat * p.splits + split] = make_float2(m_ref, dsum);
+        else if (p.lse != nullptr)
+          p.lse[flat] = dsum == 0.0f ? -INFINITY : (m_ref + log2f(dsum)) * 0.6931471805599453f;
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// Joins the partial results of a split list: one warp per row, four channels
+// per lane; O = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) d_s.
+template <typename TV>
+__global__ void __launch_bounds__(kCombineWarps * 32) sparse_combine_kernel(const SparseParams p,
+                                                                            int64_t rows) {
+  const int64_t flat = static_cast<int64_t>(blockIdx.x) * kCombineWarps + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (flat >= rows) return;
+  const float2* md = p.part_md + flat * p.splits;
+  float M = -INFINITY;
+  for (int s = 0; s < p.splits; ++s)
+    if (md[s].y != 0.0f) M = fmaxf(M, md[s].x);
+  float d = 0.0f;
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int s = 0; s < p.splits; ++s) {
+    const float2 t = md[s];
+    if (t.y == 0.0f) continue;  // saw no key
+    // m = -inf with d != 0: every score of the part was NaN.
+    const float w = t.x == -INFINITY ? 1.0f : ex2(t.x - M);
+    const float4 q =
+        *reinterpret_cast<const float4*>(p.part_o + (flat * p.splits + s) * kDim + lane * 4);
+    d = fmaf(w, t.y, d);
+    o.x = fmaf(w, q.x, o.x);
+    o.y = fmaf(w, q.y, o.y);
+    o.z = fmaf(w, q.z, o.z);
+    o.w = fmaf(w, q.w, o.w);
+  }
+  const float inv = d > 0.0f ? 1.0f / d : (d == 0.0f ? 0.0f : d);
+  const int bh = static_cast<int>(flat / p.Lq);
+  const int64_t row = flat - static_cast<int64_t>(bh) * p.Lq;
+  TV* out = static_cast<TV*>(p.out) + (bh / p.Hq) * p.o_sb + (bh % p.Hq) * p.o_sh + row * p.o_sl +
+            lane * 4;
+  *reinterpret_cast<uint2*>(out) =
+      make_uint2(pack2<TV>(o.x * inv, o.y * inv), pack2<TV>(o.z * inv, o.w * inv));
+  if (p.lse != nullptr && lane == 0)
+    p.lse[flat] = d == 0.0f ? -INFINITY : (M + log2f(d)) * 0.6931471805599453f;
+}
+
+// CTAs that share one list: as many as fill two per SM, each with at least
+// four blocks (one full ring: fewer would pay more for Q, the tile's end and
+// the join than they save).
+int split_count(int64_t tiles, int64_t keep) {
+  const int64_t slots = 2LL * device_sm_count();
+  if (tiles >= slots) return 1;
+  const int64_t s = std::max<int64_t>(1, std::min(slots / tiles, (keep + 3) / 4));
+  const int64_t chunk = (keep + s - 1) / s;
+  return static_cast<int>((keep + chunk - 1) / chunk);
+}
+
+void check_geometry(int64_t B, int64_t Hq, int64_t Lq, int64_t keep) {
+  TB_REQUIRE(B > 0 && Hq > 0 && Lq > 0, "empty Q/K sequences are not supported");
+  TB_REQUIRE(keep > 0 && keep <= (1 << 24), "block_index must name 1 to 2^24 blocks a list");
+  TB_REQUIRE(Lq <= INT32_MAX - 256, "sequence length exceeds the kernel range");
+  TB_REQUIRE(B <= INT32_MAX / Hq && B * Hq <= INT32_MAX / ((Lq + kRows - 1) / kRows),
+             "batch, heads and query blocks exceed the grid range");
+}
+
+}  // namespace
+}  // namespace tb
+
+using tb::guarded;
+
+extern "C" int tb_sparse_attn_workspace(int64_t B, int64_t Hq, int64_t Lq, int64_t keep,
+                                        int64_t* bytes) {
+  return guarded([&] {
+    TB_REQUIRE(bytes != nullptr, "the workspace size needs a place");
+    tb::check_geometry(B, Hq, Lq, keep);
+    tb::require_sm100();
+    const int splits = tb::split_count(B * Hq * ((Lq + tb::kRows - 1) / tb::kRows), keep);
+    *bytes = splits > 1 ? B * Hq * Lq * splits * (tb::kDim + 2) * 4 : 0;
+  });
+}
+
+extern "C" int tb_sparse_attn(const int8_t* q, const int8_t* k, const void* v, int v_dtype,
+                              void* out, const float* q_scale, const float* k_scale,
+                              const int32_t* block_index, const int32_t* key_lengths, float* lse,
+                              void* workspace, int64_t workspace_bytes, int64_t B, int64_t Hq,
+                              int64_t Hk, int64_t Lq, int64_t Lk, int64_t D, int64_t keep,
+                              const int64_t* strides, float sm_scale, tb_stream_t stream) {
+  return guarded([&] {
+    using namespace tb;
+    TB_REQUIRE(q && k && v && out && q_scale && k_scale && block_index && strides,
+               "query, key, value, output, scales and block_index must be CUDA tensors");
+    TB_REQUIRE(D == kDim, "the sparse attention kernel takes head_dim 128 (pad smaller heads)");
+    TB_REQUIRE(v_dtype == TB_DTYPE_BF16 || v_dtype == TB_DTYPE_F16,
+               "value must be float16 or bfloat16");
+    check_geometry(B, Hq, Lq, keep);
+    TB_REQUIRE(Hk > 0 && Lk > 0, "empty Q/K sequences are not supported");
+    TB_REQUIRE(Hq % Hk == 0, "num_qo_heads must be divisible by num_kv_heads");
+    TB_REQUIRE(Lk <= INT32_MAX - 256, "sequence length exceeds the kernel range");
+    TB_REQUIRE(std::isfinite(sm_scale), "sm_scale must be finite");
+    for (int i = 0; i < 6; ++i)
+      TB_REQUIRE(strides[i] % 16 == 0, "Q/K strides must be multiples of 16 bytes");
+    for (int i = 6; i < 12; ++i)
+      TB_REQUIRE(strides[i] % 8 == 0, "V/O strides must be multiples of 16 bytes");
+    auto aligned = [](const void* ptr, uintptr_t a) {
+      return (reinterpret_cast<uintptr_t>(ptr) & (a - 1)) == 0;
+    };
+    TB_REQUIRE(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(out, 16),
+               "Q/K/V/O must be 16-byte aligned");
+    TB_REQUIRE(aligned(q_scale, 4) && aligned(k_scale, 4) && aligned(block_index, 4) &&
+                   aligned(key_lengths, 4) && aligned(lse, 4),
+               "scales, block_index, key_lengths and lse must be 4-byte aligned");
+    require_sm100();
+    const int64_t query_blocks = (Lq + kRows - 1) / kRows;
+    const int64_t tiles = B * Hq * query_blocks;
+    SparseParams p{};
+    p.splits = split_count(tiles, keep);
+    p.chunk = static_cast<int>((keep + p.splits - 1) / p.splits);
+    if (p.splits > 1) {
+      TB_REQUIRE(workspace != nullptr && aligned(workspace, 16) &&
+                     workspace_bytes >= B * Hq * Lq * p.splits * (kDim + 2) * 4,
+                 "the split sparse attention needs the workspace tb_sparse_attn_workspace names");
+      TB_REQUIRE(tiles * p.splits <= INT32_MAX,
+                 "batch, heads and query blocks exceed the grid range");
+      p.part_o = static_cast<float*>(workspace);
+      p.part_md = reinterpret_cast<float2*>(p.part_o + B * Hq * Lq * p.splits * kDim);
+    }
+    p.Hq = static_cast<int>(Hq);
+    p.Hk = static_cast<int>(Hk);
+    p.Lq = static_cast<int>(Lq);
+    p.Lk = static_cast<int>(Lk);
+    p.groups = static_cast<int>(Hq / Hk);
+    p.query_blocks = static_cast<int>(query_blocks);
+    p.keep = static_cast<int>(keep);
+    p.q_tiles_scale = static_cast<int>((Lq + 63) / 64 * 4);
+    p.k_tiles_scale = static_cast<int>((Lk + 63) / 64);
+    p.q_scale = q_scale;
+    p.k_scale = k_scale;
+    p.lists = block_index;
+    p.key_lengths = key_lengths;
+    p.out = out;
+    p.o_sb = strides[9];
+    p.o_sh = strides[10];
+    p.o_sl = strides[11];
+    p.lse = lse;
+    p.sm_scale_log2 = sm_scale * 1.4426950408889634f;
+    CUtensorMap tq, tk, tv;
+    make_map_4d(&tq, CU_TENSOR_MAP_DATA_TYPE_UINT8, q, D, Lq, Hq, B, strides[2], strides[1],
+                strides[0], 1, kDim, kRows);
+    make_map_4d(&tk, CU_TENSOR_MAP_DATA_TYPE_UINT8, k, D, Lk, Hk, B, strides[5], strides[4],
+                strides[3], 1, kDim, kKeys);
+    make_map_4d(&tv,
+                v_dtype == TB_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                         : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                v, D, Lk, Hk, B, strides[8], strides[7], strides[6], 2, 64, kKeys);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const int64_t rows = B * Hq * Lq;
+    auto launch = [&](auto kern, auto combine) {
+      TB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         kSmemBytes));
+      kern<<<static_cast<unsigned>(tiles * p.splits), kThreads, kSmemBytes, s>>>(tq, tk, tv, p);
+      TB_CUDA_CHECK(cudaGetLastError());
+      if (p.splits > 1) {
+        combine<<<static_cast<unsigned>((rows + kCombineWarps - 1) / kCombineWarps),
+                  kCombineWarps * 32, 0, s>>>(p, rows);
+        TB_CUDA_CHECK(cudaGetLastError());
+      }
+    };
+    if (v_dtype == TB_DTYPE_BF16)
+      launch(sparse_attn_kernel<__nv_bfloat16>, sparse_combine_kernel<__nv_bfloat16>);
+    else
+      launch(sparse_attn_kernel<__half>, sparse_combine_kernel<__half>);
+  });
+}

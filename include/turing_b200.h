@@ -450,6 +450,56 @@ TB_API int tb_rope_freqs(const void *positions, int position_type, int64_t posit
                          void *output, int64_t batch, int64_t length, int64_t pairs, int dtype,
                          double scale, tb_stream_t stream);
 
+/* ------------------------------------------- block-sparse attention ---- */
+
+/* Chooses the key blocks (64 keys, one k_scale block) that each block of 128
+ * queries attends to: block_index int32 [B, Hq, ceil(Lq/128), keep], ascending,
+ * filled up with -1 where fewer blocks can be chosen.  The score of a pair is
+ * the product of the mean dequantized query and the mean dequantized visible
+ * key, exact to fp64; the keep highest are taken, ties to the lowest block, a
+ * NaN score last.  q, k: the INT8 codes of the Sage quantizers with q_scale
+ * [B, Hq, ceil(Lq/64)*4] and k_scale [B, Hk, ceil(Lk/64)]; strides (elements,
+ * 6 values): q (b, h, l), k (b, h, l), multiples of 16, last dimension
+ * contiguous, Q/K 16-byte aligned.  key_lengths int32 [B] or NULL: keys from
+ * there on are not seen (clamped to 0 .. Lk).  block_policy int8 [policy_rows,
+ * ceil(Lk/64)] or NULL, one row for all query blocks or one for each: < 0 never
+ * chosen, > 0 ranked above every score.  D = 64 or 128, 1 <= keep <=
+ * ceil(Lk/64), Lk <= 1572864.  workspace: 16-byte aligned, at least the bytes
+ * that tb_select_key_blocks_workspace returns.  No counterpart in the
+ * reference's dense path (its Sol routes score inside the attention kernel,
+ * kernel/csrc/turing/sage/sol_sparse_cuda_sm75.cu). */
+TB_API int tb_select_key_blocks_workspace(int64_t B, int64_t Hq, int64_t Hk, int64_t Lq,
+                                          int64_t Lk, int64_t D, int64_t *bytes);
+TB_API int tb_select_key_blocks(const int8_t *q, const int8_t *k, const float *q_scale,
+                                const float *k_scale, const int32_t *key_lengths,
+                                const int8_t *block_policy, int64_t policy_rows,
+                                int32_t *block_index, void *workspace, int64_t workspace_bytes,
+                                int64_t B, int64_t Hq, int64_t Hk, int64_t Lq, int64_t Lk,
+                                int64_t D, int64_t keep, const int64_t *strides,
+                                tb_stream_t stream);
+
+/* Sage attention (tb_qk_int8_sv_f16_accum_f32_attn, not causal) over the key
+ * blocks that block_index int32 [B, Hq, ceil(Lq/128), keep] names for each block
+ * of 128 queries, in any order; entries that name no block with visible keys
+ * (negative, too large, at or past key_lengths) are skipped, a block named
+ * twice counts twice.  Keys from key_lengths[b] (int32 [B] or NULL, clamped to
+ * 0 .. Lk) on are not seen, whatever K and V hold there.  A row that sees no
+ * key is 0.  out of V's dtype; lse: optional [B, Hq, Lq] natural log-sum-exp
+ * (-inf for a row that sees no key).  strides (elements, 12 values): q, k, v,
+ * out (b, h, l), Q/K multiples of 16, V/out of 8, last dimension contiguous;
+ * Q/K/V/out 16-byte aligned; D = 128.  workspace: 16-byte aligned, at least the
+ * bytes that tb_sparse_attn_workspace returns (0: may be NULL).  The sparse
+ * counterpart of the reference's attn_cuda_sm75.h:21-31 with the caller's
+ * lists in place of its Sol routes. */
+TB_API int tb_sparse_attn_workspace(int64_t B, int64_t Hq, int64_t Lq, int64_t keep,
+                                    int64_t *bytes);
+TB_API int tb_sparse_attn(const int8_t *q, const int8_t *k, const void *v, int v_dtype, void *out,
+                          const float *q_scale, const float *k_scale, const int32_t *block_index,
+                          const int32_t *key_lengths, float *lse, void *workspace,
+                          int64_t workspace_bytes, int64_t B, int64_t Hq, int64_t Hk, int64_t Lq,
+                          int64_t Lk, int64_t D, int64_t keep, const int64_t *strides,
+                          float sm_scale, tb_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
