@@ -14,7 +14,8 @@ import math
 import torch
 
 from . import _lib
-from ._lib import POSITION_TYPES, call, float_dtype_code, layout_strides, ptr, stream_of
+from ._lib import (FLOAT_CODES, POSITION_TYPES, call, device_major, float_dtype_code,
+                   layout_strides, on_device, ptr, raw_stream, stream_of)
 
 
 def _check(cond: bool, msg: str) -> None:
@@ -560,6 +561,10 @@ def turing_layer_norm_adaln(input, scale, shift, epsilon):
 
 # ----------------------------------------------------------- rotary positions
 
+_ROPE_LAYOUTS = {"HND": (_lib.TB_LAYOUT_HND, 1, 2), "NHD": (_lib.TB_LAYOUT_NHD, 2, 1)}
+_NO_STRIDES = (0, 0, 0)
+
+
 def _rope_positions(positions, inv_freq, axis_pairs, batch, length, device):
     """Checks the positions and frequencies of a rotary call; returns them as the
     kernel reads them with the number of position rows, the axes and their pairs."""
@@ -568,23 +573,27 @@ def _rope_positions(positions, inv_freq, axis_pairs, batch, length, device):
            "rotary positions and frequencies must use the input's CUDA device")
     _check(positions.dtype in POSITION_TYPES,
            "positions must be int32, int64, float32, or float64")
-    _check(inv_freq.dim() == 1 and inv_freq.numel() > 0
+    _check(inv_freq.dim() == 1 and inv_freq.size(0) > 0
            and inv_freq.dtype in (torch.float32, torch.float64),
            "inv_freq must be a 1D float32 or float64 tensor")
-    axes = 1 if axis_pairs is None else len(axis_pairs)
-    _check(1 <= axes <= 4, "positions must have 1 to 4 axes")
-    _check(axis_pairs is None or (min(axis_pairs) >= 0 and sum(axis_pairs) == inv_freq.numel()),
-           "axis_pairs must add up to the number of channel pairs")
+    shape = tuple(positions.shape)
     if axis_pairs is None:
-        positions = positions.unsqueeze(-1)
-    if positions.dim() == 2:
-        positions = positions.unsqueeze(0)
-    _check(positions.dim() == 3 and positions.size(0) in (1, batch)
-           and positions.size(1) == length and positions.size(2) == axes,
+        axes, counts = 1, None
+        lead = shape
+    else:
+        axes = len(axis_pairs)
+        _check(1 <= axes <= 4, "positions must have 1 to 4 axes")
+        _check(min(axis_pairs) >= 0 and sum(axis_pairs) == inv_freq.size(0),
+               "axis_pairs must add up to the number of channel pairs")
+        counts = (ctypes.c_int32 * axes)(*axis_pairs)
+        lead = shape[:-1] if shape and shape[-1] == axes else ()
+    rows = 1 if len(lead) == 1 else (lead[0] if len(lead) == 2 else 0)
+    _check(rows in (1, batch) and len(lead) > 0 and lead[-1] == length,
            "positions must be [L] or [1 or B, L], with a last dimension of one value per axis "
            "when axis_pairs is given")
-    counts = None if axis_pairs is None else (ctypes.c_int32 * axes)(*axis_pairs)
-    return positions.contiguous(), inv_freq.to(torch.float64).contiguous(), axes, counts
+    if inv_freq.dtype != torch.float64:
+        inv_freq = inv_freq.to(torch.float64)
+    return positions.contiguous(), inv_freq.contiguous(), rows, axes, counts
 
 
 def turing_rope(query, key, positions, inv_freq, tensor_layout="HND", split_half=False,
@@ -592,39 +601,45 @@ def turing_rope(query, key, positions, inv_freq, tensor_layout="HND", split_half
     """Rotary positions on the first 2 * len(inv_freq) channels of each head of
     query and (unless None) key, in one launch.  Returns new contiguous tensors
     (key's is None when key is).  Not a reference binding."""
-    _check(tensor_layout in ("HND", "NHD"), f"Unsupported tensor_layout: {tensor_layout}")
-    layout = _lib.TB_LAYOUT_NHD if tensor_layout == "NHD" else _lib.TB_LAYOUT_HND
-    head_axis, seq_axis = (1, 2) if layout == _lib.TB_LAYOUT_HND else (2, 1)
-    tensors = [query] if key is None else [query, key]
-    for t in tensors:
-        _check(t.is_cuda and t.dim() == 4, "rotary input must be a 4D CUDA tensor")
-        _check_float_like(t, "rotary input")
-        _check(t.device == query.device and t.dtype == query.dtype
-               and t.size(0) == query.size(0) and t.size(seq_axis) == query.size(seq_axis)
-               and t.size(3) == query.size(3),
+    if tensor_layout not in _ROPE_LAYOUTS:
+        raise RuntimeError(f"Unsupported tensor_layout: {tensor_layout}")
+    layout, head_axis, seq_axis = _ROPE_LAYOUTS[tensor_layout]
+    device, dtype = query.device, query.dtype
+    _check(query.is_cuda and query.dim() == 4, "rotary input must be a 4D CUDA tensor")
+    _check_float_like(query, "rotary input")
+    shape = query.shape
+    batch, length, head_dim = shape[0], shape[seq_axis], shape[3]
+    if key is not None:
+        _check(key.is_cuda and key.dim() == 4, "rotary input must be a 4D CUDA tensor")
+        kshape = key.shape
+        _check(key.device == device and key.dtype == dtype and kshape[0] == batch
+               and kshape[seq_axis] == length and kshape[3] == head_dim,
                "query and key must share device, dtype, batch, length, and head dimension")
-    tensors = [t if t.stride(3) == 1 or t.size(3) == 1 else t.contiguous() for t in tensors]
-    batch, length, head_dim = query.size(0), query.size(seq_axis), query.size(3)
-    rot_dim = 2 * inv_freq.numel()
-    _check(rot_dim <= head_dim, "rot_dim must be even and within the head dimension")
+    _check(2 * inv_freq.numel() <= head_dim, "rot_dim must be even and within the head dimension")
     _check(math.isfinite(scale), "scale must be finite")
-    positions, inv_freq, axes, counts = _rope_positions(positions, inv_freq, axis_pairs, batch,
-                                                        length, query.device)
-    with torch.cuda.device(query.device):
-        _require_blackwell(query.device, "rotary positions")
-        outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in tensors]
-        # A tensor without elements (no tokens, or a key without heads) takes no part.
-        live = [(t, o) for t, o in zip(tensors, outs) if t.numel() > 0]
+    positions, inv_freq, rows, axes, counts = _rope_positions(
+        positions, inv_freq, axis_pairs, batch, length, device)
+    _check(device_major(device) == 10,
+           "rotary positions requires an sm_100 (B200) device for this build")
+    with on_device(device):
+        outs, live = [], []
+        for t in (query,) if key is None else (query, key):
+            if t.stride(3) != 1 and head_dim != 1:
+                t = t.contiguous()
+            out = torch.empty_like(t, memory_format=torch.contiguous_format)
+            outs.append(out)
+            if out.numel() > 0:  # no tokens, or a key without heads: takes no part
+                live.append((t, out, layout_strides(t, layout), layout_strides(out, layout)))
         if live:
-            (t0, o0), (t1, o1) = live[0], live[1] if len(live) > 1 else (None, None)
-            strides = (ctypes.c_int64 * 12)(
-                *layout_strides(t0, layout), *(layout_strides(t1, layout) if live[1:] else (0,) * 3),
-                *layout_strides(o0, layout), *(layout_strides(o1, layout) if live[1:] else (0,) * 3))
-            call("tb_rope", ptr(t0), ptr(t1), ptr(o0), ptr(o1), ptr(positions),
-                 POSITION_TYPES[positions.dtype], positions.size(0), ptr(inv_freq), counts, axes,
-                 batch, t0.size(head_axis), t1.size(head_axis) if live[1:] else 0, length,
-                 head_dim, rot_dim, strides, int(bool(split_half)), int(bool(inverse)),
-                 float_dtype_code(query), float(scale), stream_of(query))
+            t0, o0, si0, so0 = live[0]
+            t1, o1, si1, so1 = live[1] if len(live) > 1 else (None, None, _NO_STRIDES, _NO_STRIDES)
+            call("tb_rope", t0.data_ptr(), None if t1 is None else t1.data_ptr(), o0.data_ptr(),
+                 None if o1 is None else o1.data_ptr(), positions.data_ptr(),
+                 POSITION_TYPES[positions.dtype], rows, inv_freq.data_ptr(), counts, axes, batch,
+                 t0.size(head_axis), 0 if t1 is None else t1.size(head_axis), length, head_dim,
+                 2 * inv_freq.size(0), (ctypes.c_int64 * 12)(*si0, *si1, *so0, *so1),
+                 int(bool(split_half)), int(bool(inverse)), float_dtype_code(query), float(scale),
+                 raw_stream(device))
     return (outs[0], None) if key is None else (outs[0], outs[1])
 
 
@@ -633,21 +648,23 @@ def turing_rope_freqs(positions, inv_freq, axis_pairs=None, scale=1.0, dtype=tor
     len(inv_freq), 2, 2]: the freqs operand of the fused Q/K prologue.  Not a
     reference binding."""
     _check(positions.is_cuda, "rotary positions and frequencies must use the input's CUDA device")
-    lead = positions.dim() - (0 if axis_pairs is None else 1)
-    _check(lead in (1, 2), "positions must be [L] or [1 or B, L], with a last dimension of one "
-                           "value per axis when axis_pairs is given")
-    batch, length = (1, positions.size(0)) if lead == 1 else positions.shape[:2]
-    _check(dtype in (torch.float16, torch.bfloat16, torch.float32),
-           "rotary matrices must be float16, bfloat16, or float32")
+    lead = positions.shape if axis_pairs is None else positions.shape[:-1]
+    _check(len(lead) in (1, 2), "positions must be [L] or [1 or B, L], with a last dimension of "
+                                "one value per axis when axis_pairs is given")
+    batch, length = (1, lead[0]) if len(lead) == 1 else lead
+    code = FLOAT_CODES.get(dtype)
+    _check(code is not None, "rotary matrices must be float16, bfloat16, or float32")
     _check(math.isfinite(scale), "scale must be finite")
-    dev = positions.device
-    positions, inv_freq, axes, counts = _rope_positions(positions, inv_freq, axis_pairs, batch,
-                                                        length, dev)
-    with torch.cuda.device(dev):
-        _require_blackwell(dev, "rotary positions")
-        out = torch.empty((batch, length, 1, inv_freq.numel(), 2, 2), dtype=dtype, device=dev)
+    device = positions.device
+    positions, inv_freq, rows, axes, counts = _rope_positions(positions, inv_freq, axis_pairs,
+                                                              batch, length, device)
+    _check(device_major(device) == 10,
+           "rotary positions requires an sm_100 (B200) device for this build")
+    pairs = inv_freq.size(0)
+    with on_device(device):
+        out = torch.empty((batch, length, 1, pairs, 2, 2), dtype=dtype, device=device)
         if out.numel() > 0:
-            call("tb_rope_freqs", ptr(positions), POSITION_TYPES[positions.dtype],
-                 positions.size(0), ptr(inv_freq), counts, axes, ptr(out), batch, length,
-                 inv_freq.numel(), float_dtype_code(out), float(scale), stream_of(positions))
+            call("tb_rope_freqs", positions.data_ptr(), POSITION_TYPES[positions.dtype], rows,
+                 inv_freq.data_ptr(), counts, axes, out.data_ptr(), batch, length, pairs, code,
+                 float(scale), raw_stream(device))
     return out

@@ -5,6 +5,7 @@ the shared object is missing or cannot be loaded, every entry point raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -26,6 +27,8 @@ TB_DTYPE_F16 = 1
 TB_DTYPE_F32 = 2
 TB_LAYOUT_NHD = 0
 TB_LAYOUT_HND = 1
+FLOAT_CODES = {torch.bfloat16: TB_DTYPE_BF16, torch.float16: TB_DTYPE_F16,
+               torch.float32: TB_DTYPE_F32}
 # Element types of rotary positions (TB_POS_*).
 POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2, torch.float64: 3}
 
@@ -149,10 +152,38 @@ def layout_strides(t: torch.Tensor, layout: int) -> tuple[int, int, int]:
     """(batch, head, token) element strides of a 4-D tensor in layout NHD or HND.
     A dimension of one element gets the stride that a contiguous tensor of this
     layout has: its own may be any number."""
-    _, n1, n2, d = t.shape
-    natural = (n1 * n2 * d, n2 * d, d)
-    s = [t.stride(i) if t.size(i) != 1 else natural[i] for i in range(3)]
-    return (s[0], s[2], s[1]) if layout == TB_LAYOUT_NHD else (s[0], s[1], s[2])
+    n0, n1, n2, d = t.shape
+    s0, s1, s2, _ = t.stride()
+    if n0 == 1:
+        s0 = n1 * n2 * d
+    if n1 == 1:
+        s1 = n2 * d
+    if n2 == 1:
+        s2 = d
+    return (s0, s2, s1) if layout == TB_LAYOUT_NHD else (s0, s1, s2)
+
+
+_HERE_ALREADY = contextlib.nullcontext()
+_majors: dict[int, int] = {}
+
+
+def on_device(device: torch.device):
+    """torch.cuda.device(device), skipped (1.4 us a call) where it is current."""
+    return _HERE_ALREADY if torch.cuda.current_device() == device.index else torch.cuda.device(
+        device)
+
+
+def device_major(device: torch.device) -> int:
+    """Compute capability major of a device (it never changes, so asked once)."""
+    major = _majors.get(device.index)
+    if major is None:
+        major = _majors[device.index] = torch.cuda.get_device_capability(device)[0]
+    return major
+
+
+def raw_stream(device: torch.device) -> int:
+    """Handle of the device's current stream (stream_of without its Stream object)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def stream_of(t: torch.Tensor):

@@ -11,6 +11,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.utils._python_dispatch import is_in_torch_dispatch_mode
 
 from . import _C
 
@@ -460,6 +461,61 @@ _rope_op.register_autograd(_rope_backward, setup_context=_rope_setup)
 _rope_qk_op.register_autograd(_rope_qk_backward, setup_context=_rope_setup)
 
 
+# Eager calls on plain CUDA tensors skip the custom op's dispatcher, which costs
+# more than a small launch (one token: 68 us a call through it against 21, with
+# its gradients 289 against 140): without gradients they reach the binding, with
+# gradients by way of an autograd function.  Tracing (torch.compile, fake and
+# subclass tensors, dispatch modes) sees the custom op.
+
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
+
+
+def _eager(*tensors: torch.Tensor) -> bool:
+    if torch.compiler.is_compiling() or is_in_torch_dispatch_mode():
+        return False
+    return all(type(t) in _PLAIN and t.is_cuda for t in tensors)
+
+
+class _RopeFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, query, key, positions, inv_freq, options):
+        ctx.save_for_backward(positions, inv_freq)
+        ctx.set_materialize_grads(False)
+        ctx.options = options
+        query, key = _C.turing_rope(query, key, positions, inv_freq, *options)
+        return query if key is None else (query, key)
+
+    @staticmethod
+    def backward(ctx, grad_query, grad_key=None):
+        positions, inv_freq = ctx.saved_tensors
+        options = (*ctx.options[:-1], not ctx.options[-1])
+        if not ctx.needs_input_grad[0]:
+            grad_query = None
+        if not ctx.needs_input_grad[1]:
+            grad_key = None
+        if grad_query is None:
+            if grad_key is not None:
+                grad_key = _rope_call(grad_key, None, positions, inv_freq, options)
+        elif grad_key is None:
+            grad_query = _rope_call(grad_query, None, positions, inv_freq, options)
+        else:
+            grad_query, grad_key = _rope_call(grad_query, grad_key, positions, inv_freq, options)
+        return grad_query, grad_key, None, None, None
+
+
+def _rope_call(query, key, positions, inv_freq, options):
+    if _eager(query, positions, inv_freq) if key is None else _eager(query, key, positions,
+                                                                     inv_freq):
+        if torch.is_grad_enabled() and (query.requires_grad
+                                        or (key is not None and key.requires_grad)):
+            return _RopeFunction.apply(query, key, positions, inv_freq, options)
+        rotated = _C.turing_rope(query, key, positions, inv_freq, *options)
+        return rotated[0] if key is None else rotated
+    if key is None:
+        return _rope_op(query, positions, inv_freq, *options)
+    return _rope_qk_op(query, key, positions, inv_freq, *options)
+
+
 def turing_rope(
     x: torch.Tensor,
     positions: torch.Tensor,
@@ -481,8 +537,8 @@ def turing_rope(
     [1 or B, L]; with axis_pairs (pairs of each of 1 to 4 axes) [L, axes] or
     [1 or B, L, axes].  inverse turns the other way.
     """
-    return _rope_op(x, positions, inv_freq, tensor_layout, split_half, axis_pairs, float(scale),
-                    inverse)
+    return _rope_call(x, None, positions, inv_freq,
+                      (tensor_layout, split_half, axis_pairs, float(scale), inverse))
 
 
 def turing_rope_qk(
@@ -499,8 +555,8 @@ def turing_rope_qk(
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """turing_rope of query and key (same batch, length and head dimension, any
     head counts) in one launch, differentiable in both."""
-    return _rope_qk_op(query, key, positions, inv_freq, tensor_layout, split_half, axis_pairs,
-                       float(scale), inverse)
+    return _rope_call(query, key, positions, inv_freq,
+                      (tensor_layout, split_half, axis_pairs, float(scale), inverse))
 
 
 @torch.library.custom_op("turing_utils::rope_freqs", mutates_args=())
@@ -534,4 +590,6 @@ def turing_rope_freqs(
     """The rotations of turing_rope as matrices scale * [[cos, -sin], [sin, cos]],
     [1 or B, L, 1, len(inv_freq), 2, 2]: the freqs argument of
     turing_sage.prequantize_rms_rope_qk."""
+    if _eager(positions, inv_freq):
+        return _C.turing_rope_freqs(positions, inv_freq, axis_pairs, float(scale), dtype)
     return _rope_freqs_op(positions, inv_freq, axis_pairs, float(scale), dtype)
