@@ -17,9 +17,9 @@
 // the product with k_scale_j / n_j is the first fp64 rounding.  The sum order
 // never matters, equal blocks score equal.
 //
-//   1. block_sums_kernel: 16-byte loads, channel sums as packed 16-bit lanes of
-//      the biased bytes; a warp per key block, a CTA per query block (a warp
-//      per 16-token scale tile).  HBM-bound: the only pass over Q and K.
+//   1. block_sums_kernel: 16-byte loads, channel sums by dp4a of transposed
+//      words; a warp per key block, a CTA per query block (a warp per 16-token
+//      scale tile).  HBM-bound: the only pass over Q and K.
 //   2. block_select_kernel: a CTA takes up to 8 query blocks of one key head
 //      (its query heads' blocks in a row) and all key blocks, 128 at a time:
 //      M = 128 key blocks, N = 8 query blocks x 6 digits, K = channels, twice
@@ -27,12 +27,12 @@
 //      4-stage ring, warp 9 issues the MMAs into two TMEM buffers, warps 0-3
 //      and 4-7 take the tiles in turn and leave the top word of each score's
 //      sortable bits in shared memory.  Then one warp per query block finds the
-//      keep-th word by bracketing it, and, where that word is shared by more blocks
+//      keep-th word (find_edge), and, where that word is shared by more blocks
 //      than fit, again with their low words from the digits.  Two CTAs per SM
 //      (up to 1300 key blocks): one's search runs under the other's products.
 #include <algorithm>
+#include <cmath>
 
-#define TB_TRY_WAIT_NO_HINT 1
 #include "attn_common.cuh"
 #include "tb_capi_internal.h"
 #include "tb_tu.cuh"
@@ -43,9 +43,10 @@ namespace {
 constexpr int kQueryBlock = 128;
 constexpr int kKeyBlock = 64;
 constexpr int kTileRows = 16;            // tokens of one q_scale
-constexpr int kSumThreads = 256;
+constexpr int kSumThreads = 128;
 constexpr int kSumWarps = kSumThreads / 32;
-static_assert(kSumWarps * kTileRows == kQueryBlock, "one warp per scale tile");
+constexpr int kTiles = kQueryBlock / kTileRows;
+static_assert(kTiles == 2 * kSumWarps && kSumThreads == 128, "two scale tiles per warp, a thread per channel");
 constexpr int kChannels = 128;           // of a digit plane's row (64-channel heads: half zero)
 constexpr int kQDigits = 6;
 constexpr int kKDigits = 2;
@@ -79,8 +80,10 @@ struct SelectParams {
   int q_tiles_scale;
   int rows_cta;                // query blocks per CTA, <= kMaxRows
   int groups;                  // CTAs per key head
+  float z;                     // normal quantile that `keep` of the key blocks exceed
   int8_t* q_digits;            // [B * Hq * query_blocks, kQDigits, kChannels]
   int8_t* k_digits;            // [kKDigits, B * Hk, key_blocks, kChannels]
+  double* k_factor;            // [B * Hk, key_blocks]: k_scale / visible keys
   int32_t* out;                // [B * Hq * query_blocks, keep]
 };
 
@@ -101,55 +104,58 @@ __device__ __forceinline__ int visible_keys(const SelectParams& p, int b) {
   return p.key_lengths != nullptr ? max(0, min(__ldg(p.key_lengths + b), p.Lk)) : p.Lk;
 }
 
-// Sums of the channels of 16 bytes, kept as biased (byte + 128) 16-bit lanes:
-// word w holds channels 4w and 4w + 2 in `even`, 4w + 1 and 4w + 3 in `odd`.
-struct ByteSums {
-  uint32_t even[4] = {0u, 0u, 0u, 0u}, odd[4] = {0u, 0u, 0u, 0u};
-  __device__ __forceinline__ void add(const uint4& v) {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+// Channel sums of INT8 rows: a lane owns 16 channels of every kStep-th row.
+// Four rows' words are transposed (8 byte permutes) so that one dp4a adds four
+// rows of a channel: 12 instructions per 16 bytes, a third of widening them.
+struct ChannelSums {
+  int acc[16];
+  __device__ __forceinline__ ChannelSums() {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t u = w[i] ^ 0x80808080u;
-      even[i] += u & 0x00ff00ffu;
-      odd[i] += (u >> 8) & 0x00ff00ffu;
+    for (int i = 0; i < 16; ++i) acc[i] = 0;
+  }
+  __device__ __forceinline__ void add4(uint32_t a, uint32_t b, uint32_t c, uint32_t d, int word) {
+    const uint32_t ab = __byte_perm(a, b, 0x5140), cd = __byte_perm(c, d, 0x5140);
+    const uint32_t ef = __byte_perm(a, b, 0x7362), gh = __byte_perm(c, d, 0x7362);
+    constexpr int kOnes = 0x01010101;
+    int* s = acc + 4 * word;
+    s[0] = __dp4a(static_cast<int>(__byte_perm(ab, cd, 0x5410)), kOnes, s[0]);
+    s[1] = __dp4a(static_cast<int>(__byte_perm(ab, cd, 0x7632)), kOnes, s[1]);
+    s[2] = __dp4a(static_cast<int>(__byte_perm(ef, gh, 0x5410)), kOnes, s[2]);
+    s[3] = __dp4a(static_cast<int>(__byte_perm(ef, gh, 0x7632)), kOnes, s[3]);
+  }
+  // Rows [0, n) of ROWS, all of the loads in flight; src is the lane's first row.
+  template <int ROWS, int STEP>
+  __device__ __forceinline__ void add_rows(const int8_t* src, int64_t stride, int sub, int n) {
+    constexpr int kLoads = ROWS / STEP;
+    uint4 v[(kLoads + 3) / 4 * 4];
+#pragma unroll
+    for (int i = 0; i < (kLoads + 3) / 4 * 4; ++i) {
+      v[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (i < kLoads && i * STEP + sub < n)
+        v[i] = *reinterpret_cast<const uint4*>(src + i * STEP * stride);
+    }
+#pragma unroll
+    for (int i = 0; i < kLoads; i += 4) {
+      add4(v[i].x, v[i + 1].x, v[i + 2].x, v[i + 3].x, 0);
+      add4(v[i].y, v[i + 1].y, v[i + 2].y, v[i + 3].y, 1);
+      add4(v[i].z, v[i + 1].z, v[i + 2].z, v[i + 3].z, 2);
+      add4(v[i].w, v[i + 1].w, v[i + 2].w, v[i + 3].w, 3);
     }
   }
-  // Over the lanes that hold the same channels of other rows.
+  // Over the lanes that own the same channels: pair i holds channels 2i and
+  // 2i + 1 as S1 * 2^16 + S0 (exact: both fit 16 bits signed, and sums of such
+  // pairs are pairs of sums).
   template <int LANES_PER_ROW>
-  __device__ __forceinline__ void reduce() {
+  __device__ __forceinline__ void reduce(int (&pair)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) pair[i] = acc[2 * i + 1] * 65536 + acc[2 * i];
 #pragma unroll
     for (int m = LANES_PER_ROW; m < 32; m <<= 1) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        even[i] += __shfl_xor_sync(0xffffffffu, even[i], m);
-        odd[i] += __shfl_xor_sync(0xffffffffu, odd[i], m);
-      }
+      for (int i = 0; i < 8; ++i) pair[i] += __shfl_xor_sync(0xffffffffu, pair[i], m);
     }
   }
-  // Channel c (0..15) without the bias of n rows.
-  __device__ __forceinline__ int channel(int c, int n) const {
-    const uint32_t pair = c & 1 ? odd[c >> 2] : even[c >> 2];
-    return static_cast<int>(c & 2 ? pair >> 16 : pair & 0xffffu) - 128 * n;
-  }
 };
-
-// Adds rows [0, n) of a ROWS-row tile, all of its loads in flight.
-template <int D, int ROWS>
-__device__ __forceinline__ void sum_rows(ByteSums& sums, const int8_t* src, int64_t stride, int sub,
-                                         int n) {
-  constexpr int kStep = 32 / (D / 16);
-  src += sub * stride;
-  uint4 v[ROWS / kStep];
-#pragma unroll
-  for (int i = 0; i < ROWS / kStep; ++i) {
-    // Bytes 0x80 are -128, a biased zero: rows past the end add nothing.
-    v[i] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
-    if (i * kStep + sub < n) v[i] = *reinterpret_cast<const uint4*>(src + i * kStep * stride);
-  }
-#pragma unroll
-  for (int i = 0; i < ROWS / kStep; ++i) sums.add(v[i]);
-  sums.reduce<D / 16>();
-}
 
 // Block and (batch, head) of a task, in the order that memory is laid out:
 // where a token's heads lie side by side, the heads of a block come one after
@@ -166,21 +172,19 @@ __device__ __forceinline__ void block_of(int64_t task, int B, int H, int blocks,
   }
 }
 
-__device__ __forceinline__ int low_digit(int64_t v) {
-  return static_cast<int>((v + 64) & 127) - 64;
-}
-
 template <int D>
-__global__ void __launch_bounds__(kSumThreads, 3) block_sums_kernel(const SelectParams p) {
+__global__ void __launch_bounds__(kSumThreads, 8) block_sums_kernel(const SelectParams p) {
   constexpr int kLanesPerRow = D / 16;
-  __shared__ double part[kSumWarps][kChannels];
+  __shared__ double part[kTiles][kChannels];
   __shared__ int top;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int col = (lane % kLanesPerRow) * 16;
   const int sub = lane / kLanesPerRow;
   const int64_t key_tasks = static_cast<int64_t>(p.B) * p.Hk * p.key_blocks;
   const int64_t key_ctas = (key_tasks + kSumWarps - 1) / kSumWarps;
-  ByteSums sums;
+  constexpr int kStep = 32 / kLanesPerRow;
+  ChannelSums sums;
+  int pair[8];
   if (blockIdx.x < key_ctas) {
     const int64_t task = static_cast<int64_t>(blockIdx.x) * kSumWarps + warp;
     if (task >= key_tasks) return;
@@ -189,172 +193,277 @@ __global__ void __launch_bounds__(kSumThreads, 3) block_sums_kernel(const Select
     const int b = bh / p.Hk;
     const int n = min(kKeyBlock, visible_keys(p, b) - j * kKeyBlock);
     if (n <= 0) return;  // never scored
-    sum_rows<D, kKeyBlock>(sums, p.k + b * p.k_s[0] + (bh % p.Hk) * p.k_s[1] +
-                                     static_cast<int64_t>(j) * kKeyBlock * p.k_s[2] + col,
-                           p.k_s[2], sub, n);
+    const int8_t* src = p.k + b * p.k_s[0] + (bh % p.Hk) * p.k_s[1] +
+                        static_cast<int64_t>(j) * kKeyBlock * p.k_s[2] + col;
+    const int64_t at = static_cast<int64_t>(bh) * p.key_blocks + j;
+    const float scale = __ldg(p.k_scale + at);
+    // Eight loads in flight per lane: twice as many cost occupancy.
+    constexpr int kPart = 8 * kStep;
+    static_assert(kKeyBlock % kPart == 0, "whole parts");
+    src += sub * p.k_s[2];
+#pragma unroll 1
+    for (int r = 0; r < n; r += kPart)
+      sums.add_rows<kPart, kStep>(src + r * p.k_s[2], p.k_s[2], sub, n - r);
+    sums.reduce<kLanesPerRow>(pair);
     if (sub < kKDigits) {  // lane group d writes digit plane d
-      uint32_t w[4] = {0u, 0u, 0u, 0u};
+      uint32_t w[4];
 #pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        const int s = sums.channel(c, n);
-        const int lo = low_digit(s);
-        const int digit = sub == 0 ? lo : (s - lo) >> 7;
-        w[c >> 2] |= static_cast<uint32_t>(digit & 255) << (8 * (c & 3));
+      for (int i = 0; i < 4; ++i) {
+        // S + 64 * 129 in [0, 2^14], in two 16-bit lanes each: the two digits,
+        // each plus 64.
+        const uint32_t x = static_cast<uint32_t>(pair[2 * i]) + 64u * 129u * 0x00010001u;
+        const uint32_t y = static_cast<uint32_t>(pair[2 * i + 1]) + 64u * 129u * 0x00010001u;
+        const uint32_t xd = (sub == 0 ? x & 0x007f007fu : (x >> 7) & 0x01ff01ffu) + 0x00c000c0u;
+        const uint32_t yd = (sub == 0 ? y & 0x007f007fu : (y >> 7) & 0x01ff01ffu) + 0x00c000c0u;
+        w[i] = __byte_perm(xd, yd, 0x6420);  // the low byte of every lane: minus 64 mod 256
       }
-      const int64_t at = static_cast<int64_t>(bh) * p.key_blocks + j;
       int8_t* dst = p.k_digits + (sub * key_tasks + at) * kChannels + col;
       *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
       if (D < kChannels) *reinterpret_cast<uint4*>(dst + D) = make_uint4(0, 0, 0, 0);
     }
+    if (lane == 0) p.k_factor[at] = static_cast<double>(scale) / n;
     return;
   }
   int i, bh;
   block_of(blockIdx.x - key_ctas, p.B, p.Hq, p.query_blocks, p.q_s, i, bh);
   const int64_t at = static_cast<int64_t>(bh) * p.query_blocks + i;
-  const int row0 = i * kQueryBlock + warp * kTileRows;
-  const int n = max(0, min(kTileRows, p.Lq - row0));
   if (threadIdx.x == 0) top = 0;
-  sum_rows<D, kTileRows>(sums, p.q + (bh / p.Hq) * p.q_s[0] + (bh % p.Hq) * p.q_s[1] +
-                                   row0 * p.q_s[2] + col,
-                         p.q_s[2], sub, n);
-  const double scale =
-      n > 0 ? static_cast<double>(__ldg(p.q_scale + static_cast<int64_t>(bh) * p.q_tiles_scale +
-                                        row0 / kTileRows))
-            : 0.0;
-  if (sub < 4) {  // lane group s keeps the four channels of word s
-    uint32_t e = sums.even[0], o = sums.odd[0];
+  const int8_t* src = p.q + (bh / p.Hq) * p.q_s[0] + (bh % p.Hq) * p.q_s[1] + col;
+  const float* scales = p.q_scale + static_cast<int64_t>(bh) * p.q_tiles_scale + i * kTiles;
+  ChannelSums other;
+  float scale[2];
+  // Both tiles' loads are in flight before either is added up.
 #pragma unroll
-    for (int w = 1; w < 4; ++w) {
-      e = sub == w ? sums.even[w] : e;
-      o = sub == w ? sums.odd[w] : o;
+  for (int t = 0; t < 2; ++t) {
+    const int row0 = i * kQueryBlock + (2 * warp + t) * kTileRows;
+    const int n = min(kTileRows, p.Lq - row0);
+    scale[t] = n > 0 ? __ldg(scales + 2 * warp + t) : 0.0f;
+    (t == 0 ? sums : other)
+        .add_rows<kTileRows, kStep>(src + (row0 + sub) * p.q_s[2], p.q_s[2], sub, n);
+  }
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    (t == 0 ? sums : other).reduce<kLanesPerRow>(pair);
+    if (sub < 4) {  // lane group s keeps channels 4s .. 4s + 3
+      int a = pair[0], b = pair[1];
+#pragma unroll
+      for (int w = 1; w < 4; ++w) {
+        a = sub == w ? pair[2 * w] : a;
+        b = sub == w ? pair[2 * w + 1] : b;
+      }
+      auto scaled = [&](int v) {  // v in the low mantissa bits of 2^52 + 2^31: exact
+        return static_cast<double>(scale[t]) *
+               (__hiloint2double(0x43300000, v ^ static_cast<int>(0x80000000u)) -
+                4503601774854144.0);
+      };
+      const int a0 = static_cast<int16_t>(a), b0 = static_cast<int16_t>(b);
+      // Stored by lane, 32 bytes apart: no bank conflicts.
+      double2* dst = reinterpret_cast<double2*>(
+          &part[2 * warp + t][(sub * kLanesPerRow + col / 16) * 4]);
+      dst[0] = make_double2(scaled(a0), scaled((a - a0) >> 16));
+      dst[1] = make_double2(scaled(b0), scaled((b - b0) >> 16));
     }
-    // Exact: a 16-bit sum in the low mantissa bits of 2^52.
-    const double bias = 4503599627370496.0 + 128.0 * n;
-    auto scaled = [&](uint32_t v) {
-      return scale * (__hiloint2double(0x43300000, static_cast<int>(v)) - bias);
-    };
-    double2* dst = reinterpret_cast<double2*>(&part[warp][col + sub * 4]);
-    dst[0] = make_double2(scaled(e & 0xffffu), scaled(o & 0xffffu));
-    dst[1] = make_double2(scaled(e >> 16), scaled(o >> 16));
   }
   __syncthreads();
-  const int c = threadIdx.x;
+  const int x = threadIdx.x;  // place in `part`
   double m = 0.0;
-  if (c < kChannels) {
-    if (c < D) {
+  if (x < kChannels) {
+    if (x < D) {
 #pragma unroll
-      for (int w = 0; w < kSumWarps; ++w) m += part[w][c];
+      for (int w = 0; w < kTiles; ++w) m += part[w][x];
     }
     // Exponent field of the largest channel (NaN and infinity: 0x7ff).
-    const int e = (__double2hiint(m) >> 20) & 0x7ff;
-    const int we = __reduce_max_sync(0xffffffffu, static_cast<unsigned>(e));
-    if (lane == 0) atomicMax(&top, we);
+    const unsigned e = (__double2hiint(m) >> 20) & 0x7ff;
+    const unsigned we = __reduce_max_sync(0xffffffffu, e);
+    if (lane == 0) atomicMax(&top, static_cast<int>(we));
   }
   __syncthreads();
-  if (c < kChannels) {
-    // |m| < 2^(top - 1022).  A block whose mean is not finite scores 0 everywhere.
-    int64_t v = top == 0x7ff ? 0 : llrint(ldexp(m, kFixBits - (top - 1022)));
+  if (x < kChannels) {
+    // |m| < 2^(top - 1022); v = m * 2^(kFixBits + 1022 - top) to the nearest
+    // integer, by the rounding of an addition to 1.5 * 2^52.  (fp32 scales keep
+    // top above 800.)  A block whose mean is not finite scores 0 everywhere.
+    int64_t v = 0;
+    if (top > 64 && top < 0x7ff) {
+      const double unit = __hiloint2double((1023 + kFixBits + 1022 - top) << 20, 0);
+      const double magic = 6755399441055744.0;
+      v = __double_as_longlong(fma(m, unit, magic)) - __double_as_longlong(magic);
+    }
+    // Digits plus 64 of v + 64 (128^6 - 1) / 127.
+    const uint64_t u = static_cast<uint64_t>(v + 64 * ((1ll << (7 * kQDigits)) - 1) / 127);
+    const int c = x < D ? (x / 4 % kLanesPerRow) * 16 + x / (4 * kLanesPerRow) * 4 + x % 4 : x;
     int8_t* dst = p.q_digits + at * (kQDigits * kChannels) + c;
 #pragma unroll
-    for (int d = 0; d < kQDigits; ++d) {
-      const int digit = low_digit(v);
-      dst[d * kChannels] = static_cast<int8_t>(digit);
-      v = (v - digit) >> 7;
-    }
+    for (int d = 0; d < kQDigits; ++d)
+      dst[d * kChannels] = static_cast<int8_t>(static_cast<int>((u >> (7 * d)) & 127) - 64);
   }
 }
 
-// Orders fp64 scores as unsigned integers, -0 as 0 and NaN as -infinity; below
-// every score lies 0 (a block that cannot be chosen), above it ~0.
-__device__ __forceinline__ uint64_t sort_key(double score) {
-  if (isnan(score)) score = -INFINITY;
-  const int64_t bits = __double_as_longlong(score + 0.0);
-  return bits < 0 ? ~static_cast<uint64_t>(bits)
-                  : static_cast<uint64_t>(bits) | 0x8000000000000000ull;
+// score = v * factor as a sortable 64-bit integer: -0 as 0, NaN as -infinity;
+// below every score lies 0 (a block that cannot be chosen), above it ~0.  v is
+// converted by two exact pieces and one rounding (the conversion unit would
+// bound the kernel).
+__device__ __forceinline__ double exact_score(int64_t v, double factor) {
+  const double hi = __hiloint2double(0x45300000, static_cast<int>(v >> 32) ^ 0x80000000);
+  const double lo = __hiloint2double(0x43300000, static_cast<int>(v));
+  const double x = (hi - 19342822341709703277445120.0) + lo;  // 2^84 + 2^63 + 2^52
+  return fma(x, factor, 0.0);
+}
+__device__ __forceinline__ uint32_t top_word(double score) {
+  uint32_t hi = static_cast<uint32_t>(__double2hiint(score));
+  if ((hi & 0x7fffffffu) > 0x7ff00000u) hi = 0xfff00000u;  // NaN
+  return hi ^ (static_cast<uint32_t>(static_cast<int>(hi) >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ uint32_t low_word(double score) {
+  const uint32_t lo = static_cast<uint32_t>(__double2loint(score));
+  return isnan(score) ? 0xffffffffu : (__double2hiint(score) < 0 ? ~lo : lo);
 }
 
-__device__ __forceinline__ double block_factor(const SelectParams& p, int64_t kv, int j, int n) {
-  return static_cast<double>(__ldg(p.k_scale + kv * p.key_blocks + j)) / n;
+// The score that a key starts, to fp32's range and precision, and back.  Only
+// used to guess.
+__device__ __forceinline__ float key_value(uint32_t key) {
+  const uint32_t hi = key & 0x80000000u ? key ^ 0x80000000u : ~key;
+  const int mag = static_cast<int>(hi & 0x7fffffffu) - (896 << 20);
+  const int fit = max(0, min(mag, 0x0fdfffff));
+  return __uint_as_float((hi & 0x80000000u) | (static_cast<uint32_t>(fit) << 3));
+}
+__device__ __forceinline__ uint32_t value_key(float x) {
+  const uint32_t bits = __float_as_uint(x);
+  const uint32_t hi = (bits & 0x80000000u) | (((bits & 0x7fffffffu) >> 3) + (896u << 20));
+  return hi ^ (static_cast<uint32_t>(static_cast<int>(hi) >> 31) | 0x80000000u);
 }
 
-struct Edge {
-  uint32_t word;  // the keep-th highest key
-  int left;       // keys equal to it that are kept, lowest first
-  bool shared;    // more keys equal it than are kept
-};
-
-// Score whose sort key starts with `word`.
-__device__ __forceinline__ double key_score(uint32_t word) {
-  return __hiloint2double(
-      static_cast<int>(word & 0x80000000u ? word ^ 0x80000000u : ~word), 0);
-}
-
-// The keep-th highest of n keys, the warp together; with no more than `keep`
-// keys above 0 all of those are kept.  Brackets the edge between two keys whose
-// counts enclose `keep` and shrinks the bracket: by interpolating the counts
-// over the scores, by the middle score, and by the middle key, which alone
-// would end after 32 steps (scores of one row: 8 steps instead of 22).  The
-// first PER_LANE * 32 keys stay in registers; longer rows read shared memory.
+// The `keep` highest of a row's n keys: their places into out, ascending, equals
+// lowest first, -1 where fewer keys are above 0; the warp together.  Returns
+// false, with the edge, where more keys equal the edge than fit and `settle` is
+// not set (the caller then refines the keys).
+//
+// The edge: a bracket of two keys whose counts enclose `keep` is shrunk until a
+// threshold counts exactly `keep` or one key is left.  The first guess is the
+// normal quantile (`z`) of the scores' mean and deviation, the next interpolate
+// the counts (an end that stays twice counts half); after 12 the middle key,
+// which needs at most 32 more.  About 6 thresholds a row; halving the key range
+// took 22.  The first PER_LANE * 32 keys stay in registers (four counters hide
+// the compare-and-add latency), longer rows read shared memory.
 template <int PER_LANE>
-__device__ __forceinline__ Edge find_edge(const uint32_t* row, int n, int keep) {
+__device__ __forceinline__ bool choose_row(const uint32_t* row, int n, int keep, float z,
+                                           bool settle, int32_t* out, uint32_t& edge) {
   const int lane = static_cast<int>(lane_id());
   uint32_t own[PER_LANE];
   const int rest = PER_LANE * 32 + lane;
-  uint32_t low = ~0u, top = 0u;  // of the keys that scores gave
-  int total = 0, ranked = 0;     // keys above 0; keys above every score
-  auto see = [&](uint32_t key) {
-    total += key != 0u;
-    ranked += key == ~0u;
-    if (key != 0u) low = min(low, key);
-    if (key != ~0u) top = max(top, key);
-  };
 #pragma unroll
-  for (int i = 0; i < PER_LANE; ++i) {
-    own[i] = i * 32 + lane < n ? row[i * 32 + lane] : 0u;
-    see(own[i]);
-  }
-#pragma unroll 4
-  for (int j = rest; j < n; j += 32) see(row[j]);
+  for (int i = 0; i < PER_LANE; ++i) own[i] = i * 32 + lane < n ? row[i * 32 + lane] : 0u;
   auto sum = [](int v) {
     return static_cast<int>(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(v)));
   };
-  total = sum(total);
-  ranked = sum(ranked);
-  if (total <= keep) return {1u, keep, false};
-  if (ranked >= keep) return {~0u, keep, ranked > keep};
-  uint32_t lo = __reduce_min_sync(0xffffffffu, low);
-  uint32_t hi = __reduce_max_sync(0xffffffffu, top) + 1u;  // top < ~0
-  int above_lo = total, above_hi = ranked;  // keys >= lo (> keep), >= hi (< keep)
-  for (int step = 0; hi - lo > 1u; ++step) {
-    uint32_t t = lo + (hi - lo) / 2;
-    if ((step & 3) != 3) {
-      const double a = key_score(lo), b = key_score(hi);
-      const double part = step & 1 ? 0.5
-                                   : static_cast<double>(above_lo - keep) /
-                                         static_cast<double>(above_lo - above_hi);
-      const uint32_t guess = static_cast<uint32_t>(sort_key(a + (b - a) * part) >> 32);
-      if (guess > lo && guess < hi) t = guess;
-    }
-    int count = 0;
+  auto reach = [&](uint32_t t) {  // keys >= t
+    int c[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < PER_LANE; ++i) count += own[i] >= t;
+    for (int i = 0; i < PER_LANE; ++i) c[i & 3] += own[i] >= t ? 1 : 0;
 #pragma unroll 4
-    for (int j = rest; j < n; j += 32) count += row[j] >= t;
-    count = sum(count);
-    if (count == keep) return {t, keep, false};
-    if (count > keep) {
-      lo = t;
-      above_lo = count;
-    } else {
-      hi = t;
-      above_hi = count;
+    for (int j = rest; j < n; j += 32) c[0] += row[j] >= t ? 1 : 0;
+    return sum((c[0] + c[1]) + (c[2] + c[3]));
+  };
+  int left = keep;  // equals of the edge that are kept
+  const int total = reach(1u), ranked = reach(~0u);
+  if (total <= keep) {
+    edge = 1u;
+  } else if (ranked >= keep) {
+    edge = ~0u;
+  } else {
+    uint32_t low[2] = {~0u, ~0u}, top[2] = {0u, 0u};  // of the keys that scores gave
+#pragma unroll
+    for (int i = 0; i < PER_LANE; ++i) {
+      low[i & 1] = min(low[i & 1], own[i] - 1u);  // 0 wraps to the end
+      top[i & 1] = max(top[i & 1], own[i] + 1u);  // ~0 wraps to the start
+    }
+    for (int j = rest; j < n; j += 32) {
+      low[0] = min(low[0], row[j] - 1u);
+      top[0] = max(top[0], row[j] + 1u);
+    }
+    uint32_t lo = __reduce_min_sync(0xffffffffu, min(low[0], low[1])) + 1u;
+    uint32_t hi = __reduce_max_sync(0xffffffffu, max(top[0], top[1]));
+    int above_lo = total, above_hi = ranked;  // keys >= lo (> keep), >= hi (< keep)
+    float sx = 0.0f, sxx = 0.0f;
+    const float base = key_value(lo);
+    // A quarter of the keys (every fourth 32) is sample enough.
+#pragma unroll
+    for (int i = 0; i < PER_LANE; i += 4) {
+      const float x = own[i] + 1u > 1u ? key_value(own[i]) - base : 0.0f;
+      sx += x;
+      sxx = fmaf(x, x, sxx);
+    }
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) {
+      sx += __shfl_xor_sync(0xffffffffu, sx, m);
+      sxx += __shfl_xor_sync(0xffffffffu, sxx, m);
+    }
+    const float part = 4.0f / static_cast<float>(min(n, PER_LANE * 32) + 127);
+    const float mean = sx * part;
+    float guess = base + mean + z * sqrtf(fmaxf(0.0f, sxx * part - mean * mean));
+    float half_lo = 1.0f, half_hi = 1.0f;
+    int last = 0;
+    bool exact = false;
+    for (int step = 0; hi - lo > 1u; ++step) {
+      uint32_t t = lo + (hi - lo) / 2;
+      if (step < 12) {
+        const uint32_t g = value_key(guess);
+        if (g > lo && g < hi) t = g;
+      }
+      const int c = reach(t);
+      if (c == keep) {
+        lo = t;
+        exact = true;
+        break;
+      }
+      if (c > keep) {
+        lo = t;
+        above_lo = c;
+        half_lo = 1.0f;
+        if (last == 1) half_hi *= 0.5f;
+        last = 1;
+      } else {
+        hi = t;
+        above_hi = c;
+        half_hi = 1.0f;
+        if (last == -1) half_lo *= 0.5f;
+        last = -1;
+      }
+      const float a = key_value(lo), b = key_value(hi);
+      const float fa = static_cast<float>(above_lo - keep) * half_lo;
+      const float fb = static_cast<float>(keep - above_hi) * half_hi;
+      guess = a + (b - a) * __fdividef(fa, fa + fb);
+    }
+    edge = lo;
+    if (!exact) {
+      if (!settle) return false;
+      left = keep - above_hi;
     }
   }
-  return {lo, keep - above_hi, true};
+  const uint32_t before = (1u << lane) - 1u;
+  int count = 0;
+  auto emit = [&](uint32_t key, int j) {
+    bool take = key >= edge;
+    if (left < keep) {  // the edge is shared
+      const bool equal = key == edge;
+      const uint32_t equals = __ballot_sync(0xffffffffu, equal);
+      take = key > edge || (equal && __popc(equals & before) < left);
+      left = max(left - __popc(equals), -keep);
+    }
+    const uint32_t taken = __ballot_sync(0xffffffffu, take);
+    const int at = count + __popc(taken & before);
+    if (take && at < keep) out[at] = j;
+    count += __popc(taken);
+  };
+#pragma unroll
+  for (int i = 0; i < PER_LANE; ++i)
+    if (i * 32 < n) emit(own[i], i * 32 + lane);
+  for (int j = rest; j - lane < n; j += 32) emit(j < n ? row[j] : 0u, j);
+  for (int j = count + lane; j < keep; j += 32) out[j] = -1;
+  return true;
 }
 
-constexpr int kRegisterKeys = 40;  // per lane: rows up to 1280 key blocks
-
+// PER_LANE: keys of a row that a lane of the search keeps in registers.
+template <int PER_LANE>
 __global__ void __launch_bounds__(kSelectThreads, 2)
     block_select_kernel(const __grid_constant__ CUtensorMap tm_q,
                         const __grid_constant__ CUtensorMap tm_k, const SelectParams p) {
@@ -454,10 +563,12 @@ __global__ void __launch_bounds__(kSelectThreads, 2)
   } else {
     // Warps 0-3 take the even tiles, 4-7 the odd ones: one key block per thread.
     const int buf = warp >> 2, quad = warp & 3;
-    for (int t = buf; t < tiles; t += 2) {
-      const int j = t * kTileKeys + quad * 32 + lane;
-      const int n = min(kKeyBlock, key_len - j * kKeyBlock);
-      const double factor = n > 0 ? block_factor(p, kv, j, n) : 0.0;
+    const double* factors = p.k_factor + kv * p.key_blocks;
+    int j = buf * kTileKeys + quad * 32 + lane;
+    double next_factor = j < blocks ? factors[j] : 0.0;
+    for (int t = buf; t < tiles; t += 2, j += 2 * kTileKeys) {
+      const double factor = next_factor;
+      if (j + 2 * kTileKeys < blocks) next_factor = factors[j + 2 * kTileKeys];
       if (!__all_sync(0xffffffffu,
                       mbar_wait(&bar->tmem_full[buf], static_cast<uint32_t>(t >> 1) & 1u,
                                 abort_flag, kDevWaitTimeoutEpilogue)))
@@ -492,8 +603,8 @@ __global__ void __launch_bounds__(kSelectThreads, 2)
                             static_cast<int64_t>(w[5] * 128 + w[4]) * (1ll << 28) +
                             static_cast<int64_t>(w[6]) * (1ll << 42);
           const int r = r0 + i;
-          if (n > 0 && r < rows) {
-            uint32_t key = static_cast<uint32_t>(sort_key(static_cast<double>(v) * factor) >> 32);
+          if (j < blocks && r < rows) {
+            uint32_t key = top_word(exact_score(v, factor));
             if (p.policy != nullptr) {
               const int prow = p.policy_rows == 1 ? 0 : (row_in_head + r) % p.query_blocks;
               const int pol = p.policy[static_cast<int64_t>(prow) * p.key_blocks + j];
@@ -518,63 +629,58 @@ __global__ void __launch_bounds__(kSelectThreads, 2)
 
   uint32_t* row = keys + static_cast<int64_t>(warp) * blocks;
   const int64_t grow = row0 + warp;
-  Edge edge = find_edge<kRegisterKeys>(row, blocks, p.keep);
-  if (edge.shared && edge.word != ~0u) {
-    // Blocks share the edge's top word: their low words decide.  The digits give
-    // the same integer, so the same fp64 score, as the tensor core did.
-    const int8_t* qd = p.q_digits + grow * (kQDigits * kChannels) + lane * 4;
-    int64_t q[4];
+  int32_t* out = p.out + grow * p.keep;
+  uint32_t edge = 0u;
+  if (choose_row<PER_LANE>(row, blocks, p.keep, p.z, false, out, edge)) return;
+  // Blocks share the edge's top word: their low words decide.  The digits give
+  // the same integer, so the same fp64 score, as the tensor core did.
+  const int8_t* qd = p.q_digits + grow * (kQDigits * kChannels) + lane * 4;
+  int64_t q[4];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      q[c] = 0;
+  for (int c = 0; c < 4; ++c) {
+    q[c] = 0;
 #pragma unroll
-      for (int d = kQDigits - 1; d >= 0; --d) q[c] = q[c] * 128 + qd[d * kChannels + c];
-    }
-    const int64_t plane = static_cast<int64_t>(p.B) * p.Hk * p.key_blocks * kChannels;
-    for (int j = 0; j < blocks; ++j) {
-      const uint32_t word = row[j];
-      uint32_t next = word > edge.word ? ~0u : 0u;
-      if (word == edge.word) {
-        const int8_t* kd = p.k_digits + (kv * p.key_blocks + j) * kChannels + lane * 4;
-        int64_t v = 0;
+    for (int d = kQDigits - 1; d >= 0; --d) q[c] = q[c] * 128 + qd[d * kChannels + c];
+  }
+  const int64_t plane = static_cast<int64_t>(p.B) * p.Hk * p.key_blocks * kChannels;
+  for (int j = 0; j < blocks; ++j) {
+    const uint32_t word = row[j];
+    uint32_t next = word > edge ? ~0u : 0u;
+    if (word == edge) {
+      const int8_t* kd = p.k_digits + (kv * p.key_blocks + j) * kChannels + lane * 4;
+      int64_t v = 0;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) v += q[c] * (kd[plane + c] * 128 + kd[c]);
+      for (int c = 0; c < 4; ++c) v += q[c] * (kd[plane + c] * 128 + kd[c]);
 #pragma unroll
-        for (int m = 16; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
-        const int n = min(kKeyBlock, key_len - j * kKeyBlock);
-        const uint64_t full = sort_key(static_cast<double>(v) * block_factor(p, kv, j, n));
-        next = 1u + (static_cast<uint32_t>(full) >> 1);
-      }
-      __syncwarp();
-      if (lane == 0) row[j] = next;
+      for (int m = 16; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+      next = 1u + (low_word(exact_score(v, p.k_factor[kv * p.key_blocks + j])) >> 1);
     }
     __syncwarp();
-    edge = find_edge<kRegisterKeys>(row, blocks, p.keep);
+    if (lane == 0) row[j] = next;
   }
-  int32_t* out = p.out + grow * p.keep;
-  const uint32_t before = (1u << lane) - 1u;
-  int count = 0, left = edge.left;
-  for (int j0 = 0; j0 < blocks; j0 += 32) {
-    const int j = j0 + lane;
-    const uint32_t key = j < blocks ? row[j] : 0u;
-    const bool equal = key == edge.word;
-    const uint32_t equals = __ballot_sync(0xffffffffu, equal);
-    const bool take = key > edge.word || (equal && __popc(equals & before) < left);
-    const uint32_t taken = __ballot_sync(0xffffffffu, take);
-    if (take) out[count + __popc(taken & before)] = j;
-    count += __popc(taken);
-    left -= min(left, __popc(equals));
+  __syncwarp();
+  choose_row<PER_LANE>(row, blocks, p.keep, p.z, true, out, edge);
+}
+
+// Quantile of the standard normal distribution by bisection of erfc: a guess's
+// precision is enough.
+float normal_quantile(double q) {
+  double lo = -6.0, hi = 6.0;
+  for (int i = 0; i < 24; ++i) {
+    const double x = 0.5 * (lo + hi);
+    (0.5 * std::erfc(-x * 0.70710678118654752) < q ? lo : hi) = x;
   }
-  for (int j = count + lane; j < p.keep; j += 32) out[j] = -1;
+  return static_cast<float>(lo);
 }
 
 struct SelectWorkspace {
-  int64_t q_bytes, k_bytes;
+  int64_t q_bytes, k_bytes, factor_bytes;
+  int64_t total() const { return q_bytes + k_bytes + factor_bytes; }
 };
 SelectWorkspace select_workspace(int64_t B, int64_t Hq, int64_t Hk, int64_t Lq, int64_t Lk) {
   const int64_t qb = (Lq + kQueryBlock - 1) / kQueryBlock;
   const int64_t kb = (Lk + kKeyBlock - 1) / kKeyBlock;
-  return {B * Hq * qb * kQDigits * kChannels, B * Hk * kb * kKDigits * kChannels};
+  return {B * Hq * qb * kQDigits * kChannels, B * Hk * kb * kKDigits * kChannels, B * Hk * kb * 8};
 }
 
 void check_select(int64_t B, int64_t Hq, int64_t Hk, int64_t Lq, int64_t Lk, int64_t D) {
@@ -622,12 +728,17 @@ void select_launch(SelectParams& p, cudaStream_t stream) {
                       CU_TENSOR_MAP_SWIZZLE_128B);
   }
   const size_t smem = smem_of(p.rows_cta);
-  TB_CUDA_CHECK(cudaFuncSetAttribute(block_select_kernel,
-                                     cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     static_cast<int>(smem)));
-  block_select_kernel<<<static_cast<unsigned>(heads * p.groups), kSelectThreads, smem, stream>>>(
-      tq, tk, p);
-  TB_CUDA_CHECK(cudaGetLastError());
+  auto launch = [&](auto kern) {
+    TB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       static_cast<int>(smem)));
+    kern<<<static_cast<unsigned>(heads * p.groups), kSelectThreads, smem, stream>>>(tq, tk, p);
+    TB_CUDA_CHECK(cudaGetLastError());
+  };
+  // As many register keys as a row needs; past 40 a lane the kernel would spill
+  // and the rest of a row is read from shared memory.
+  if (p.key_blocks <= 8 * 32) launch(block_select_kernel<8>);
+  else if (p.key_blocks <= 16 * 32) launch(block_select_kernel<16>);
+  else launch(block_select_kernel<40>);
 }
 
 }  // namespace
@@ -641,7 +752,7 @@ extern "C" int tb_select_key_blocks_workspace(int64_t B, int64_t Hq, int64_t Hk,
     TB_REQUIRE(bytes != nullptr, "the workspace size needs a place");
     tb::check_select(B, Hq, Hk, Lq, Lk, D);
     const tb::SelectWorkspace w = tb::select_workspace(B, Hq, Hk, Lq, Lk);
-    *bytes = w.q_bytes + w.k_bytes;
+    *bytes = w.total();
   });
 }
 
@@ -663,7 +774,7 @@ extern "C" int tb_select_key_blocks(const int8_t* q, const int8_t* k, const floa
     TB_REQUIRE(block_policy == nullptr || policy_rows == 1 || policy_rows == query_blocks,
                "block_policy must have one row or one row per query block");
     const SelectWorkspace w = select_workspace(B, Hq, Hk, Lq, Lk);
-    TB_REQUIRE(workspace_bytes >= w.q_bytes + w.k_bytes,
+    TB_REQUIRE(workspace_bytes >= w.total(),
                "the block choice needs the workspace tb_select_key_blocks_workspace names");
     auto aligned = [](const void* ptr, uintptr_t a) {
       return (reinterpret_cast<uintptr_t>(ptr) & (a - 1)) == 0;
@@ -699,6 +810,8 @@ extern "C" int tb_select_key_blocks(const int8_t* q, const int8_t* k, const floa
     p.q_tiles_scale = static_cast<int>((Lq + 63) / 64 * 4);
     p.q_digits = static_cast<int8_t*>(workspace);
     p.k_digits = p.q_digits + w.q_bytes;
+    p.k_factor = reinterpret_cast<double*>(p.k_digits + w.k_bytes);
+    p.z = normal_quantile(1.0 - (keep - 0.5) / static_cast<double>(key_blocks));
     p.out = block_index;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int64_t key_ctas = (B * Hk * key_blocks + kSumWarps - 1) / kSumWarps;
