@@ -80,7 +80,8 @@ struct SelectParams {
   int q_tiles_scale;
   int rows_cta;                // query blocks per CTA, <= kMaxRows
   int groups;                  // CTAs per key head
-  float z;                     // normal quantile that `keep` of the key blocks exceed
+  float z, slope;              // normal quantile that `keep` of the key blocks exceed; deviations
+                               // that one block more or less moves it there
   int8_t* q_digits;            // [B * Hq * query_blocks, kQDigits, kChannels]
   int8_t* k_digits;            // [kKDigits, B * Hk, key_blocks, kChannels]
   double* k_factor;            // [B * Hk, key_blocks]: k_scale / visible keys
@@ -332,63 +333,55 @@ __device__ __forceinline__ uint32_t value_key(float x) {
   return hi ^ (static_cast<uint32_t>(static_cast<int>(hi) >> 31) | 0x80000000u);
 }
 
+// Keys of a row that each lane of its search owns: an odd number, so that the
+// lanes' first keys lie in different banks.
+__host__ __device__ constexpr int keys_per_lane(int n) { return ((n + 31) / 32) | 1; }
+
 // The `keep` highest of a row's n keys: their places into out, ascending, equals
 // lowest first, -1 where fewer keys are above 0; the warp together.  Returns
 // false, with the edge, where more keys equal the edge than fit and `settle` is
-// not set (the caller then refines the keys).
+// not set (the caller then refines the keys).  Lane l owns keys l per .. (l + 1)
+// per - 1 (zeros past n), the first PER_LANE of them in registers.
 //
-// The edge: a bracket of two keys whose counts enclose `keep` is shrunk until a
-// threshold counts exactly `keep` or one key is left.  The first guess is the
-// normal quantile (`z`) of the scores' mean and deviation, the next interpolate
-// the counts (an end that stays twice counts half); after 12 the middle key,
-// which needs at most 32 more.  About 6 thresholds a row; halving the key range
-// took 22.  The first PER_LANE * 32 keys stay in registers (four counters hide
-// the compare-and-add latency), longer rows read shared memory.
+// The edge: thresholds are counted (four counters hide the compare-and-add
+// latency) until one counts exactly `keep` or the bracket holds one key.  The
+// first guess is the normal quantile (`z`) of the scores' mean and deviation;
+// until both ends of the bracket are scores it moves by the count's error over
+// the normal density (`slope`), then interpolates the counts (an end that stays
+// twice counts half); after 12 steps the middle key, which needs at most 32
+// more.  About 6 thresholds a row; halving the key range took 22.
 template <int PER_LANE>
 __device__ __forceinline__ bool choose_row(const uint32_t* row, int n, int keep, float z,
-                                           bool settle, int32_t* out, uint32_t& edge) {
+                                           float slope, bool settle, int32_t* out,
+                                           uint32_t& edge) {
   const int lane = static_cast<int>(lane_id());
+  const int per = keys_per_lane(n);
+  const int first = lane * per;
   uint32_t own[PER_LANE];
-  const int rest = PER_LANE * 32 + lane;
 #pragma unroll
-  for (int i = 0; i < PER_LANE; ++i) own[i] = i * 32 + lane < n ? row[i * 32 + lane] : 0u;
+  for (int i = 0; i < PER_LANE; ++i) own[i] = i < per ? row[first + i] : 0u;
   auto sum = [](int v) {
     return static_cast<int>(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(v)));
   };
-  auto reach = [&](uint32_t t) {  // keys >= t
+  int mine = 0;  // of the keys that `reach` counted last, this lane's
+  auto reach = [&](uint32_t t) {
     int c[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < PER_LANE; ++i) c[i & 3] += own[i] >= t ? 1 : 0;
-#pragma unroll 4
-    for (int j = rest; j < n; j += 32) c[0] += row[j] >= t ? 1 : 0;
-    return sum((c[0] + c[1]) + (c[2] + c[3]));
+    for (int i = PER_LANE; i < per; ++i) c[0] += row[first + i] >= t ? 1 : 0;
+    mine = (c[0] + c[1]) + (c[2] + c[3]);
+    return sum(mine);
   };
   int left = keep;  // equals of the edge that are kept
-  const int total = reach(1u), ranked = reach(~0u);
-  if (total <= keep) {
-    edge = 1u;
-  } else if (ranked >= keep) {
-    edge = ~0u;
-  } else {
-    uint32_t low[2] = {~0u, ~0u}, top[2] = {0u, 0u};  // of the keys that scores gave
+  bool exact = false;
+  if (n > keep) {
+    // A few keys of every lane are sample enough.
+    float sx = 0.0f, sxx = 0.0f, used = 0.0f;
 #pragma unroll
-    for (int i = 0; i < PER_LANE; ++i) {
-      low[i & 1] = min(low[i & 1], own[i] - 1u);  // 0 wraps to the end
-      top[i & 1] = max(top[i & 1], own[i] + 1u);  // ~0 wraps to the start
-    }
-    for (int j = rest; j < n; j += 32) {
-      low[0] = min(low[0], row[j] - 1u);
-      top[0] = max(top[0], row[j] + 1u);
-    }
-    uint32_t lo = __reduce_min_sync(0xffffffffu, min(low[0], low[1])) + 1u;
-    uint32_t hi = __reduce_max_sync(0xffffffffu, max(top[0], top[1]));
-    int above_lo = total, above_hi = ranked;  // keys >= lo (> keep), >= hi (< keep)
-    float sx = 0.0f, sxx = 0.0f;
-    const float base = key_value(lo);
-    // A quarter of the keys (every fourth 32) is sample enough.
-#pragma unroll
-    for (int i = 0; i < PER_LANE; i += 4) {
-      const float x = own[i] + 1u > 1u ? key_value(own[i]) - base : 0.0f;
+    for (int i = 0; i < PER_LANE; i += (PER_LANE + 7) / 8) {
+      const bool in = own[i] + 1u > 1u;  // a score: neither 0 nor ~0
+      const float x = in ? key_value(own[i]) : 0.0f;
+      used += in ? 1.0f : 0.0f;
       sx += x;
       sxx = fmaf(x, x, sxx);
     }
@@ -396,13 +389,17 @@ __device__ __forceinline__ bool choose_row(const uint32_t* row, int n, int keep,
     for (int m = 16; m > 0; m >>= 1) {
       sx += __shfl_xor_sync(0xffffffffu, sx, m);
       sxx += __shfl_xor_sync(0xffffffffu, sxx, m);
+      used += __shfl_xor_sync(0xffffffffu, used, m);
     }
-    const float part = 4.0f / static_cast<float>(min(n, PER_LANE * 32) + 127);
+    const float part = __fdividef(1.0f, used);
     const float mean = sx * part;
-    float guess = base + mean + z * sqrtf(fmaxf(0.0f, sxx * part - mean * mean));
+    const float dev = sqrtf(fmaxf(0.0f, sxx * part - mean * mean));
+    float guess = mean + z * dev;
+    uint32_t lo = 0u, hi = ~0u;            // counts > keep at lo, <= at hi ...
+    int above_lo = n, above_hi = 0;
+    bool seen_lo = false, seen_hi = false;  // ... each once it was counted
     float half_lo = 1.0f, half_hi = 1.0f;
     int last = 0;
-    bool exact = false;
     for (int step = 0; hi - lo > 1u; ++step) {
       uint32_t t = lo + (hi - lo) / 2;
       if (step < 12) {
@@ -418,48 +415,104 @@ __device__ __forceinline__ bool choose_row(const uint32_t* row, int n, int keep,
       if (c > keep) {
         lo = t;
         above_lo = c;
+        seen_lo = true;
         half_lo = 1.0f;
         if (last == 1) half_hi *= 0.5f;
         last = 1;
       } else {
         hi = t;
         above_hi = c;
+        seen_hi = true;
         half_hi = 1.0f;
         if (last == -1) half_lo *= 0.5f;
         last = -1;
       }
-      const float a = key_value(lo), b = key_value(hi);
-      const float fa = static_cast<float>(above_lo - keep) * half_lo;
-      const float fb = static_cast<float>(keep - above_hi) * half_hi;
-      guess = a + (b - a) * __fdividef(fa, fa + fb);
+      if (seen_lo && seen_hi) {
+        const float a = key_value(lo), b = key_value(hi);
+        const float fa = static_cast<float>(above_lo - keep) * half_lo;
+        const float fb = static_cast<float>(keep - above_hi) * half_hi;
+        guess = a + (b - a) * __fdividef(fa, fa + fb);
+      } else {
+        guess += static_cast<float>(c - keep + last) * slope * dev;
+      }
     }
     edge = lo;
     if (!exact) {
-      if (!settle) return false;
-      left = keep - above_hi;
+      // One key is left: `lo`, or ~0 (blocks before any score) where hi stayed
+      // there uncounted.
+      if (!seen_hi) {
+        above_hi = reach(~0u);
+        if (above_hi >= keep) {
+          edge = ~0u;
+          above_hi = 0;
+        }
+      }
+      if (edge != 0u) {
+        if (edge != ~0u && !settle) return false;
+        left = keep - above_hi;
+      }
+    }
+  } else {
+    edge = 0u;
+  }
+  if (edge == 0u) {  // no more than `keep` keys are above 0: all of those
+    edge = 1u;
+    exact = true;
+    reach(edge);
+  }
+  // Places of this lane's kept keys: after those of the lanes before it.
+  int equal = 0;
+  if (!exact) {
+    int c = 0, e = 0;
+    for (int i = 0; i < per; ++i) {
+      const uint32_t key = row[first + i];
+      c += key > edge ? 1 : 0;
+      e += key == edge ? 1 : 0;
+    }
+    int before = e;  // equals of this lane and the lanes before it
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, before, m);
+      if (lane >= m) before += v;
+    }
+    equal = max(0, min(e, left - (before - e)));
+    mine = c + equal;
+  }
+  int at = mine;
+#pragma unroll
+  for (int m = 1; m < 32; m <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, at, m);
+    if (lane >= m) at += v;
+  }
+  const int total = __shfl_sync(0xffffffffu, at, 31);
+  at -= mine;
+  if (exact) {
+#pragma unroll
+    for (int i = 0; i < PER_LANE; ++i)
+      if (own[i] >= edge) out[at++] = first + i;
+    for (int i = PER_LANE; i < per; ++i)
+      if (row[first + i] >= edge) out[at++] = first + i;
+  } else {
+    for (int i = 0; i < per; ++i) {
+      const uint32_t key = row[first + i];
+      if (key > edge || (key == edge && equal > 0)) {
+        equal -= key == edge ? 1 : 0;
+        out[at++] = first + i;
+      }
     }
   }
-  const uint32_t before = (1u << lane) - 1u;
-  int count = 0;
-  auto emit = [&](uint32_t key, int j) {
-    bool take = key >= edge;
-    if (left < keep) {  // the edge is shared
-      const bool equal = key == edge;
-      const uint32_t equals = __ballot_sync(0xffffffffu, equal);
-      take = key > edge || (equal && __popc(equals & before) < left);
-      left = max(left - __popc(equals), -keep);
-    }
-    const uint32_t taken = __ballot_sync(0xffffffffu, take);
-    const int at = count + __popc(taken & before);
-    if (take && at < keep) out[at] = j;
-    count += __popc(taken);
-  };
-#pragma unroll
-  for (int i = 0; i < PER_LANE; ++i)
-    if (i * 32 < n) emit(own[i], i * 32 + lane);
-  for (int j = rest; j - lane < n; j += 32) emit(j < n ? row[j] : 0u, j);
-  for (int j = count + lane; j < keep; j += 32) out[j] = -1;
+  for (int j = total + lane; j < keep; j += 32) out[j] = -1;
   return true;
+}
+
+__device__ __forceinline__ int64_t mad_wide(int a, int b, int c) {
+  int64_t d;
+  asm("mad.wide.s32 %0, %1, %2, %3;" : "=l"(d) : "r"(a), "r"(b), "l"(static_cast<int64_t>(c)));
+  return d;
+}
+// Keeps uses of a tmem_ld4's registers behind the tmem_wait_ld before it.
+__device__ __forceinline__ void after_wait(uint32_t (&r)[4]) {
+  asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]));
 }
 
 // PER_LANE: keys of a row that a lane of the search keeps in registers.
@@ -470,7 +523,7 @@ __global__ void __launch_bounds__(kSelectThreads, 2)
   extern __shared__ __align__(1024) unsigned char smem[];
   unsigned char* ring = smem + kQTileBytes;
   SelectBarriers* bar = reinterpret_cast<SelectBarriers*>(ring + kStages * kStageBytes);
-  uint32_t* keys = reinterpret_cast<uint32_t*>(bar + 1);  // [rows][visible blocks]
+  uint32_t* keys = reinterpret_cast<uint32_t*>(bar + 1);  // [rows][row_keys], zeros past `blocks`
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t kv = blockIdx.x / p.groups;               // (batch, key head)
@@ -482,6 +535,7 @@ __global__ void __launch_bounds__(kSelectThreads, 2)
   const int key_len = visible_keys(p, b);
   const int blocks = (key_len + kKeyBlock - 1) / kKeyBlock;
   int tiles = (blocks + kTileKeys - 1) / kTileKeys;
+  const int row_keys = 32 * keys_per_lane(blocks);
 
   if (threadIdx.x == 0) {
     mbar_init(&bar->q_full, 1);
@@ -504,6 +558,8 @@ __global__ void __launch_bounds__(kSelectThreads, 2)
   if (warp == kMmaWarp) {
     tmem_alloc(&bar->tmem_base, kTmemCols);
     tmem_relinquish();
+  } else if (warp < rows) {
+    for (int j = blocks + lane; j < row_keys; j += 32) keys[warp * row_keys + j] = 0u;
   }
   tc_fence_before();
   __syncthreads();
@@ -584,34 +640,32 @@ __global__ void __launch_bounds__(kSelectThreads, 2)
           tmem_ld4(src + d * kMaxRows + r0, lo[d]);
           tmem_ld4(src + kMmaN + d * kMaxRows + r0, hi[d]);
         }
+        tmem_wait_ld();
 #pragma unroll
         for (int d = 0; d < kQDigits; ++d) {
-          tmem_wait_ld_regs4(lo[d]);
-          tmem_wait_ld_regs4(hi[d]);
+          after_wait(lo[d]);
+          after_wait(hi[d]);
         }
+        uint32_t* dst = keys + r0 * row_keys + j;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          // Digit sums of weight 128^w, two to a 32-bit integer, in int64.
-          int w[kQDigits + 1];
-          w[0] = static_cast<int>(lo[0][i]);
-#pragma unroll
-          for (int d = 1; d < kQDigits; ++d)
-            w[d] = static_cast<int>(lo[d][i]) + static_cast<int>(hi[d - 1][i]);
-          w[kQDigits] = static_cast<int>(hi[kQDigits - 1][i]);
-          const int64_t v = static_cast<int64_t>(w[1] * 128 + w[0]) +
-                            static_cast<int64_t>(w[3] * 128 + w[2]) * (1ll << 14) +
-                            static_cast<int64_t>(w[5] * 128 + w[4]) * (1ll << 28) +
-                            static_cast<int64_t>(w[6]) * (1ll << 42);
-          const int r = r0 + i;
-          if (j < blocks && r < rows) {
-            uint32_t key = top_word(exact_score(v, factor));
-            if (p.policy != nullptr) {
-              const int prow = p.policy_rows == 1 ? 0 : (row_in_head + r) % p.query_blocks;
-              const int pol = p.policy[static_cast<int64_t>(prow) * p.key_blocks + j];
-              key = pol < 0 ? 0u : (pol > 0 ? ~0u : key);
-            }
-            keys[static_cast<int64_t>(r) * blocks + j] = key;
-          }
+          // Digit sums of weight 128^w, two to a 32-bit integer, four to an int64.
+          const int w0 = lo[0][i], w1 = lo[1][i] + hi[0][i], w2 = lo[2][i] + hi[1][i],
+                    w3 = lo[3][i] + hi[2][i], w4 = lo[4][i] + hi[3][i], w5 = lo[5][i] + hi[4][i],
+                    w6 = hi[5][i];
+          const int64_t low = mad_wide(w3 * 128 + w2, 1 << 14, w1 * 128 + w0);
+          const int64_t high = mad_wide(w6, 1 << 14, w5 * 128 + w4);
+          const uint32_t key =
+              top_word(exact_score(low + static_cast<int64_t>(static_cast<uint64_t>(high) << 28),
+                                   factor));
+          if (j < blocks && r0 + i < rows) dst[i * row_keys] = key;
+        }
+      }
+      if (p.policy != nullptr && j < blocks) {
+        for (int r = 0; r < rows; ++r) {
+          const int prow = p.policy_rows == 1 ? 0 : (row_in_head + r) % p.query_blocks;
+          const int pol = p.policy[static_cast<int64_t>(prow) * p.key_blocks + j];
+          if (pol != 0) keys[r * row_keys + j] = pol < 0 ? 0u : ~0u;
         }
       }
       tc_fence_before();
@@ -627,11 +681,11 @@ __global__ void __launch_bounds__(kSelectThreads, 2)
   }
   if (warp >= rows || *abort_flag) return;
 
-  uint32_t* row = keys + static_cast<int64_t>(warp) * blocks;
+  uint32_t* row = keys + warp * row_keys;
   const int64_t grow = row0 + warp;
   int32_t* out = p.out + grow * p.keep;
   uint32_t edge = 0u;
-  if (choose_row<PER_LANE>(row, blocks, p.keep, p.z, false, out, edge)) return;
+  if (choose_row<PER_LANE>(row, blocks, p.keep, p.z, p.slope, false, out, edge)) return;
   // Blocks share the edge's top word: their low words decide.  The digits give
   // the same integer, so the same fp64 score, as the tensor core did.
   const int8_t* qd = p.q_digits + grow * (kQDigits * kChannels) + lane * 4;
@@ -659,18 +713,18 @@ __global__ void __launch_bounds__(kSelectThreads, 2)
     if (lane == 0) row[j] = next;
   }
   __syncwarp();
-  choose_row<PER_LANE>(row, blocks, p.keep, p.z, true, out, edge);
+  choose_row<PER_LANE>(row, blocks, p.keep, p.z, p.slope, true, out, edge);
 }
 
 // Quantile of the standard normal distribution by bisection of erfc: a guess's
 // precision is enough.
-float normal_quantile(double q) {
+double normal_quantile(double q) {
   double lo = -6.0, hi = 6.0;
   for (int i = 0; i < 24; ++i) {
     const double x = 0.5 * (lo + hi);
     (0.5 * std::erfc(-x * 0.70710678118654752) < q ? lo : hi) = x;
   }
-  return static_cast<float>(lo);
+  return lo;
 }
 
 struct SelectWorkspace {
@@ -703,7 +757,7 @@ void select_launch(SelectParams& p, cudaStream_t stream) {
   const int64_t head_rows = static_cast<int64_t>(p.Hq) / p.Hk * p.query_blocks;
   const int64_t heads = static_cast<int64_t>(p.B) * p.Hk;
   auto smem_of = [&](int rows) {
-    return static_cast<size_t>(kFixedSmem) + static_cast<size_t>(rows) * p.key_blocks * 4;
+    return static_cast<size_t>(kFixedSmem) + static_cast<size_t>(rows) * 32 * keys_per_lane(p.key_blocks) * 4;
   };
   p.rows_cta = kMaxRows;
   while (p.rows_cta > 1 &&
@@ -734,11 +788,12 @@ void select_launch(SelectParams& p, cudaStream_t stream) {
     kern<<<static_cast<unsigned>(heads * p.groups), kSelectThreads, smem, stream>>>(tq, tk, p);
     TB_CUDA_CHECK(cudaGetLastError());
   };
-  // As many register keys as a row needs; past 40 a lane the kernel would spill
+  // As many register keys as a row needs; past 41 a lane the kernel would spill
   // and the rest of a row is read from shared memory.
-  if (p.key_blocks <= 8 * 32) launch(block_select_kernel<8>);
-  else if (p.key_blocks <= 16 * 32) launch(block_select_kernel<16>);
-  else launch(block_select_kernel<40>);
+  const int per_lane = keys_per_lane(p.key_blocks);
+  if (per_lane <= 9) launch(block_select_kernel<9>);
+  else if (per_lane <= 17) launch(block_select_kernel<17>);
+  else launch(block_select_kernel<41>);
 }
 
 }  // namespace
@@ -811,7 +866,9 @@ extern "C" int tb_select_key_blocks(const int8_t* q, const int8_t* k, const floa
     p.q_digits = static_cast<int8_t*>(workspace);
     p.k_digits = p.q_digits + w.q_bytes;
     p.k_factor = reinterpret_cast<double*>(p.k_digits + w.k_bytes);
-    p.z = normal_quantile(1.0 - (keep - 0.5) / static_cast<double>(key_blocks));
+    const double z = normal_quantile(1.0 - (keep - 0.5) / static_cast<double>(key_blocks));
+    p.z = static_cast<float>(z);
+    p.slope = static_cast<float>(2.5066282746310002 * std::exp(0.5 * z * z) / key_blocks);
     p.out = block_index;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int64_t key_ctas = (B * Hk * key_blocks + kSumWarps - 1) / kSumWarps;
