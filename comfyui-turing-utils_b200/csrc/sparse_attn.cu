@@ -6,7 +6,7 @@
 //   s     = S_int * (sm_scale * log2 e * q_scale[row / 16] * k_scale[key / 64])
 //   p = 2^(s - m), d = sum_L p, O = sum_L p V, out = O / d, lse = ln sum_L e^..
 // with the running reference m of one pass over the list (moved, and O and d
-// rescaled, only when a row's max grows by more than 2^8 over it).  A row that
+// rescaled, only when a row's max grows far beyond it).  A row that
 // sees no key gives 0 and lse = -inf.  S, m, d and O are INT32 / fp32; p is
 // rounded to V's 16-bit type for the second contraction (half a step 2^-9 bf16,
 // 2^-12 fp16 relative, averaged over the keys: below the output's own
@@ -19,19 +19,29 @@
 // barrier waits and tile ends filled by the other:
 //   warps 0-3  softmax, one query row per thread (TMEM lane quadrant = warp);
 //   warp 4     TMA producer: Q once, then K (8 KB) and V (16 KB) of the listed
-//              blocks into a 4-stage ring (128B swizzle);
+//              blocks into two 4-stage rings (128B swizzle): K is read two
+//              blocks before V, so one ring for both would hold a slot for
+//              three blocks and leave one to hide the loads' latency;
 //   warp 5     MMA issuer: S = Q K_j^T into one of two S buffers, O += P V_j.
 // TMEM columns: O [0, 128), S(b) at 128 + 64 b; P(j) overwrites the first 32
 // columns of its S buffer.  While the softmax turns S(j) into P, the tensor
 // core computes S(j + 1).
 //
+// The softmax is bound by the latency of its own steps: of 1440 clocks a block
+// and warp (one CTA per SM) the exponentials took 770 (their unit needs 512).
+// So what can overlap them does: the second half of S loads under the first
+// half's exponentials and the first half of the next block's S while P is stored,
+// the producer follows the list and fetches the K scales, the issuer has looked
+// at the rings before P comes, and everything rare is out of the way.
+//
 // Few query blocks (single tokens): the list is split over CTAs, which write
 // unnormalized O, m and d; sparse_combine_kernel joins them.
 //
 // List entries that name no block with visible keys (negative, or at or past
-// the end) are skipped by every role alike: the producer and softmax warps walk
-// the list 32 entries at a time with a warp vote, and the count the prologue
-// takes bounds all loops.  A block named twice counts twice.
+// the end) are skipped: the producer walks the list 32 entries at a time with a
+// warp vote and leaves each block's K scale and visible keys in a ring of notes
+// for the softmax; the count the prologue takes bounds all loops.  A block named
+// twice counts twice.
 #define TB_TRY_WAIT_NO_HINT 1
 #include <algorithm>
 #include <cmath>
@@ -47,15 +57,18 @@ constexpr int kRows = 128;   // query block
 constexpr int kKeys = 64;    // key block
 constexpr int kDim = 128;
 constexpr int kStages = 4;
+// Slot j % kNotes is written with K(j), which waits for S(j - 4), so for P(j - 6):
+// the softmax has read the slot's last note, j - 8.
+constexpr int kNotes = 8;
 constexpr int kSoftmaxWarps = 4;
 constexpr int kProducerWarp = 4;
 constexpr int kMmaWarp = 5;
 constexpr int kThreads = 192;
+constexpr int kQuarter = kKeys / 4;
 constexpr int kQBytes = kRows * kDim;
 constexpr int kKBytes = kKeys * kDim;
 constexpr int kVBytes = kKeys * kDim * 2;
-constexpr int kStageBytes = kKBytes + kVBytes;
-constexpr int kDataBytes = kQBytes + kStages * kStageBytes;
+constexpr int kDataBytes = kQBytes + kStages * (kKBytes + kVBytes);
 constexpr uint32_t kTmemCols = 256;
 constexpr uint32_t kSBase = 128;
 constexpr int kCombineWarps = 4;
@@ -76,15 +89,21 @@ struct SparseParams {
   float2* part_md;              // [B * Hq * Lq, splits] (m, d)
 };
 
+struct BlockNote {  // what the softmax has to know of a listed block
+  float k_scale;
+  int valid;        // visible keys, 1 .. 64
+};
+
 struct __align__(8) SparseBarriers {
   uint64_t q_full;
-  uint64_t kv_full[kStages];
-  uint64_t kv_empty[kStages];
+  uint64_t k_full[kStages], k_empty[kStages];
+  uint64_t v_full[kStages], v_empty[kStages];
   uint64_t s_full[2];   // S buffer b computed
   uint64_t p_full[2];   // the 4 softmax warps stored P in buffer b
   uint64_t o_done;      // after each of the last two PVs
   uint64_t o_final;     // after the last PV
   uint64_t drain;
+  BlockNote note[kNotes];
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -114,27 +133,39 @@ struct ListCursor {
   }
 };
 
-// p = 2^(s c - m) of the 64 scores of a block, in place as packed pairs of
-// V's type; `sum2` gathers the unrounded p.  Returns the integer row max where
-// TRACK_MAX.  MASKED zeroes keys >= valid.  WAIT_HI: columns 32..63 are still
-// loading.
-template <typename TV, bool TRACK_MAX, bool MASKED, bool WAIT_HI>
-__device__ __forceinline__ int exp_scores(uint32_t (&v)[kKeys], uint64_t c2, uint64_t nm2,
-                                          int valid, uint64_t (&sum2)[2]) {
-  int m[4] = {INT32_MIN, INT32_MIN, INT32_MIN, INT32_MIN};
+// How far (log2) a row's max may grow over the reference point before O and d
+// are rescaled: p stays within V's 16-bit type and the sums within fp32.
+template <typename TV>
+__device__ constexpr float kGrowth = std::is_same<TV, __nv_bfloat16>::value ? 32.0f : 12.0f;
+
+// p = 2^(s c - m) of 32 scores of a block, 16 in x and 16 in y; the packed pairs
+// of V's type replace x, y is free.  `sum2` gathers the unrounded p.  Returns
+// the integer row max where TRACK_MAX.  MASKED zeroes keys >= valid.
+template <typename TV, bool TRACK_MAX, bool MASKED>
+__device__ __forceinline__ int exp_scores(uint32_t (&x)[kQuarter], uint32_t (&y)[kQuarter],
+                                          uint64_t c2, uint64_t nm2, int valid,
+                                          uint64_t (&sum2)[2]) {
+  int m[2] = {INT32_MIN, INT32_MIN};
 #pragma unroll
-  for (int i = 0; i < kKeys / 2; ++i) {
-    if (WAIT_HI && i == kKeys / 4) tmem_wait_ld_regs(*reinterpret_cast<uint32_t(*)[32]>(v + 32));
-    if (TRACK_MAX)
-      m[i & 3] =
-          __vimax3_s32(m[i & 3], static_cast<int>(v[2 * i]), static_cast<int>(v[2 * i + 1]));
-    uint64_t p2 = ex2_pair(f2_fma(score_pair_f32(v[2 * i], v[2 * i + 1]), c2, nm2));
+  for (int i = 0; i < kQuarter; ++i) {
+    const uint32_t s0 = i < kQuarter / 2 ? x[2 * i] : y[2 * i - kQuarter];
+    const uint32_t s1 = i < kQuarter / 2 ? x[2 * i + 1] : y[2 * i + 1 - kQuarter];
+    if (TRACK_MAX) m[i & 1] = __vimax3_s32(m[i & 1], static_cast<int>(s0), static_cast<int>(s1));
+    uint64_t p2 = ex2_pair(f2_fma(score_pair_f32(s0, s1), c2, nm2));
     if (MASKED)
       p2 = f2_pack(2 * i < valid ? f2_lo(p2) : 0.0f, 2 * i + 1 < valid ? f2_hi(p2) : 0.0f);
     sum2[i & 1] = f2_add(sum2[i & 1], p2);
-    v[i] = pack_pair<TV>(p2);
+    x[i] = pack_pair<TV>(p2);
   }
-  return max(max(m[0], m[1]), max(m[2], m[3]));
+  return max(m[0], m[1]);
+}
+
+// Keeps uses of loaded registers behind the tmem_wait_ld before it.
+__device__ __forceinline__ void after_wait(uint32_t (&r)[kQuarter]) {
+  asm volatile(""
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                 "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
 }
 
 template <typename TV>
@@ -143,7 +174,8 @@ __global__ void __launch_bounds__(kThreads, 2)
                        const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v, const SparseParams p) {
   extern __shared__ __align__(1024) unsigned char smem[];
-  unsigned char* kv_smem = smem + kQBytes;
+  unsigned char* k_smem = smem + kQBytes;
+  unsigned char* v_smem = k_smem + kStages * kKBytes;
   SparseBarriers* bar = reinterpret_cast<SparseBarriers*>(smem + kDataBytes);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -165,8 +197,10 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (threadIdx.x == 0) {
     mbar_init(&bar->q_full, 1);
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(&bar->kv_full[s], 1);
-      mbar_init(&bar->kv_empty[s], 1);
+      mbar_init(&bar->k_full[s], 1);
+      mbar_init(&bar->k_empty[s], 1);
+      mbar_init(&bar->v_full[s], 1);
+      mbar_init(&bar->v_empty[s], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar->s_full[i], 1);
@@ -210,215 +244,273 @@ __global__ void __launch_bounds__(kThreads, 2)
         tma_load_4d(smem, &tm_q, &bar->q_full, 0, q0, h, b);
       }
       ListCursor cur(list, n_list, visible);
-      int stage = 0, issued = 0;
-      uint32_t phase = 0;
-      for (int j = 0; j < n_kv; ++j) {
-        const int blk = cur.next();
-        bool ok = true;
-        if (lane == 0) {
-          ok = mbar_wait(&bar->kv_empty[stage], phase ^ 1u, abort_flag, kDevWaitTimeoutProducer);
-          if (ok) {
-            unsigned char* k_dst = kv_smem + stage * kStageBytes;
-            unsigned char* v_dst = k_dst + kKBytes;
-            mbar_arrive_expect_tx(&bar->kv_full[stage], kStageBytes);
-            tma_load_4d(k_dst, &tm_k, &bar->kv_full[stage], 0, blk * kKeys, hk, b);
+      const float* ks_row = p.k_scale + static_cast<int64_t>(b * p.Hk + hk) * p.k_tiles_scale;
+      auto load_k = [&](int j, int blk) {
+        const int s = j % kStages;
+        if (!mbar_wait(&bar->k_empty[s], (static_cast<uint32_t>(j / kStages) & 1u) ^ 1u,
+                       abort_flag, kDevWaitTimeoutProducer))
+          return false;
+        bar->note[j % kNotes] = {__ldg(ks_row + blk), min(kKeys, key_len - blk * kKeys)};
+        mbar_arrive_expect_tx(&bar->k_full[s], kKBytes);  // releases the note
+        tma_load_4d(k_smem + s * kKBytes, &tm_k, &bar->k_full[s], 0, blk * kKeys, hk, b);
+        return true;
+      };
+      auto load_v = [&](int j, int blk) {
+        const int s = j % kStages;
+        if (!mbar_wait(&bar->v_empty[s], (static_cast<uint32_t>(j / kStages) & 1u) ^ 1u,
+                       abort_flag, kDevWaitTimeoutProducer))
+          return false;
+        mbar_arrive_expect_tx(&bar->v_full[s], kVBytes);
 #pragma unroll
-            for (int dh = 0; dh < kDim / 64; ++dh)
-              tma_load_4d(v_dst + dh * (kKeys * 128), &tm_v, &bar->kv_full[stage], dh * 64,
-                          blk * kKeys, hk, b);
-          }
+        for (int dh = 0; dh < kDim / 64; ++dh)
+          tma_load_4d(v_smem + s * kVBytes + dh * (kKeys * 128), &tm_v, &bar->v_full[s], dh * 64,
+                      blk * kKeys, hk, b);
+        return true;
+      };
+      // K runs two blocks ahead of V, as S does of PV.
+      int blk0 = 0, blk1 = 0, blk2 = 0, k_issued = 0, v_issued = 0;
+      for (int j = -2; j < n_kv; ++j) {
+        blk0 = blk1;
+        blk1 = blk2;
+        bool ok = true;
+        if (j + 2 < n_kv) {
+          blk2 = cur.next();
+          if (lane == 0) ok = load_k(j + 2, blk2);
+          k_issued += ok;
+        }
+        if (j >= 0 && lane == 0 && ok) {
+          ok = load_v(j, blk0);
+          v_issued += ok;
         }
         if (!__shfl_sync(0xffffffffu, static_cast<int>(ok), 0)) break;
-        ++issued;
-        if (++stage == kStages) {
-          stage = 0;
-          phase ^= 1u;
-        }
       }
       if (lane == 0) {
         // Every copy issued by this CTA lands before it exits.
         drain_wait(&bar->q_full, 0);
-        for (int i = min(issued, kStages); i > 0; --i) {
-          if (--stage < 0) {
-            stage = kStages - 1;
-            phase ^= 1u;
-          }
-          drain_wait(&bar->kv_full[stage], phase);
-        }
+        for (int i = max(0, k_issued - kStages); i < k_issued; ++i)
+          drain_wait(&bar->k_full[i % kStages], static_cast<uint32_t>(i / kStages) & 1u);
+        for (int i = max(0, v_issued - kStages); i < v_issued; ++i)
+          drain_wait(&bar->v_full[i % kStages], static_cast<uint32_t>(i / kStages) & 1u);
       }
     }
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------ MMA issuer
-    if (lane == 0 && n_kv > 0) {
+    if (n_kv > 0) {
+      const uint32_t elected = elect_one();
       constexpr uint32_t idesc_qk = idesc_i8(kRows, kKeys);
       constexpr uint32_t idesc_pv = idesc_f16(
           kRows, kDim, std::is_same<TV, __nv_bfloat16>::value, /*b_mn_major=*/true);
-      const uint32_t kv_addr = smem_u32(kv_smem);
+      const uint32_t k_addr = smem_u32(k_smem), v_addr = smem_u32(v_smem);
       const uint64_t q_desc = umma_desc_sw128(smem_u32(smem));
       auto issue_s = [&](int j) {
         const uint32_t d_tmem = tmem + kSBase + static_cast<uint32_t>(j & 1) * kKeys;
-        const uint64_t bk = umma_desc_sw128(kv_addr + (j % kStages) * kStageBytes);
+        const uint64_t bk = umma_desc_sw128(k_addr + (j % kStages) * kKBytes);
 #pragma unroll
         for (int kk = 0; kk < kDim / 32; ++kk)
-          mma_i8_ss(d_tmem, q_desc + 2u * kk, bk + 2u * kk, idesc_qk, kk > 0 ? 1u : 0u);
+          mma_i8_ss_warp(d_tmem, q_desc + 2u * kk, bk + 2u * kk, idesc_qk, kk > 0 ? 1u : 0u,
+                         elected);
       };
-      auto wait_kv = [&](int j) {
-        return mbar_wait(&bar->kv_full[j % kStages], static_cast<uint32_t>(j / kStages) & 1u,
-                         abort_flag, kDevWaitTimeoutMma);
+      auto warp_wait = [&](uint64_t* b, uint32_t parity) {
+        return __all_sync(0xffffffffu, mbar_wait(b, parity, abort_flag, kDevWaitTimeoutMma)) != 0;
       };
-      bool ok = mbar_wait(&bar->q_full, 0, abort_flag, kDevWaitTimeoutMma);
+      auto wait_ring = [&](uint64_t* full, int j) {
+        return warp_wait(&full[j % kStages], static_cast<uint32_t>(j / kStages) & 1u);
+      };
+      bool ok = warp_wait(&bar->q_full, 0);
       for (int j = 0; j < 2 && j < n_kv && ok; ++j) {
-        ok = wait_kv(j);
+        ok = wait_ring(bar->k_full, j);
         if (ok) {
           tc_fence_after();
           issue_s(j);
-          mma_commit(&bar->s_full[j & 1]);
+          mma_commit_warp(&bar->s_full[j & 1], elected);
+          mma_commit_warp(&bar->k_empty[j % kStages], elected);
         }
       }
-      // Both waits of a block first, then PV(j) and S(j + 2) back to back, then
+      // All waits of a block first, then PV(j) and S(j + 2) back to back, then
       // the commits.  The s_full commit of S(j + 2) also says that PV(j) is
       // done; o_done marks the last two PVs, which no S commit follows.
       for (int j = 0; j < n_kv && ok; ++j) {
         const bool next_s = j + 2 < n_kv;
-        ok = mbar_wait(&bar->p_full[j & 1], static_cast<uint32_t>(j >> 1) & 1u, abort_flag,
-                       kDevWaitTimeoutMma) &&
-             (!next_s || wait_kv(j + 2));
+        ok = wait_ring(bar->v_full, j) && (!next_s || wait_ring(bar->k_full, j + 2)) &&
+             warp_wait(&bar->p_full[j & 1], static_cast<uint32_t>(j >> 1) & 1u);
         if (!ok) break;
         tc_fence_after();
-        const int stage = j % kStages;
-        const uint32_t v_addr = kv_addr + stage * kStageBytes + kKBytes;
+        const uint32_t v_tile = v_addr + (j % kStages) * kVBytes;
         const uint32_t p_tmem = tmem + kSBase + static_cast<uint32_t>(j & 1) * kKeys;
 #pragma unroll
         for (int kk = 0; kk < kKeys / 16; ++kk) {
-          const uint64_t bv = umma_desc_sw128_mn(v_addr + kk * 2048, kKeys * 128, 1024);
-          mma_f16_ts(tmem, p_tmem + static_cast<uint32_t>(kk * 8), bv, idesc_pv,
-                     (j > 0 || kk > 0) ? 1u : 0u);
+          const uint64_t bv = umma_desc_sw128_mn(v_tile + kk * 2048, kKeys * 128, 1024);
+          mma_f16_ts_warp(tmem, p_tmem + static_cast<uint32_t>(kk * 8), bv, idesc_pv,
+                          (j > 0 || kk > 0) ? 1u : 0u, elected);
         }
         if (next_s) {
           issue_s(j + 2);
-          mma_commit(&bar->s_full[j & 1]);
+          mma_commit_warp(&bar->s_full[j & 1], elected);
+          mma_commit_warp(&bar->k_empty[(j + 2) % kStages], elected);
         } else {
-          mma_commit(&bar->o_done);
+          mma_commit_warp(&bar->o_done, elected);
         }
-        mma_commit(&bar->kv_empty[stage]);
-        if (j + 1 == n_kv) mma_commit(&bar->o_final);
+        mma_commit_warp(&bar->v_empty[j % kStages], elected);
+        if (j + 1 == n_kv) mma_commit_warp(&bar->o_final, elected);
       }
-      mma_commit(&bar->drain);
-      drain_wait(&bar->drain, 0);
+      mma_commit_warp(&bar->drain, elected);
+      if (lane == 0) drain_wait(&bar->drain, 0);
+      __syncwarp();
     }
-  } else {
+  } else if (warp < kSoftmaxWarps) {
     // ------------------------------------------------------------ softmax
     const int row = q0 + warp * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(warp * 32) << 16;
     const uint32_t s_tmem0 = tmem + lane_off + kSBase;
     const uint32_t o_tmem = tmem + lane_off;
-    const float* ks_row = p.k_scale + static_cast<int64_t>(b * p.Hk + hk) * p.k_tiles_scale;
     const float cq = row < p.Lq ? p.sm_scale_log2 * __ldg(p.q_scale + static_cast<int64_t>(bh) *
                                                               p.q_tiles_scale + row / 16)
                                 : 0.0f;
     float m_ref = -INFINITY;  // exponent reference point
     float dsum = 0.0f;
     bool ok = n_kv > 0;
-    ListCursor cur(list, n_list, visible);
-    int blk_next = ok ? cur.next() : 0;
-    float ks = ok ? __ldg(ks_row + blk_next) : 0.0f;
-    // tcgen05.ld / st are warp-collective: every branch around one is taken by
-    // a warp vote.
-    for (int j = 0; j < n_kv && ok; ++j) {
-      const int key0 = blk_next * kKeys;
-      const float c = cq * ks;
-      if (j + 1 < n_kv) {
-        blk_next = cur.next();
-        ks = __ldg(ks_row + blk_next);
-      }
-      ok = __all_sync(0xffffffffu,
-                      mbar_wait(&bar->s_full[j & 1], static_cast<uint32_t>(j >> 1) & 1u,
-                                abort_flag, kDevWaitTimeoutSoftmax));
-      if (!ok) break;
-      tc_fence_after();
+    bool primed = false;  // every row of the warp has a reference point
+    bool loaded = false;  // keys 0-31 of this block's S and its note were fetched by the last one
+    BlockNote note{0.0f, kKeys};
+    // One block: keys 0-31 in (l1, l2), 32-63 in (h1, h2), 16 each.  Their packed
+    // P stays in l1 and h1, so h2 and l2 are free for keys 0-31 of the next block,
+    // whose call therefore gets (h2, l2, h1, l1).  The usual path has no branch
+    // but the loop's and the one of the vote; the rest is kept out of its way.
+    auto block = [&](int j, uint32_t(&l1)[kQuarter], uint32_t(&l2)[kQuarter],
+                     uint32_t(&h1)[kQuarter], uint32_t(&h2)[kQuarter]) {
       const uint32_t s_tmem = s_tmem0 + static_cast<uint32_t>(j & 1) * kKeys;
-      const int valid = min(kKeys, key_len - key0);  // >= 1, the same for every row
-      uint32_t v[kKeys];
-      tmem_ld32(s_tmem, *reinterpret_cast<uint32_t(*)[32]>(v));
-      tmem_wait_ld_regs(*reinterpret_cast<uint32_t(*)[32]>(v));
-      tmem_ld32(s_tmem + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
+      if (__builtin_expect(!loaded, 0)) {
+        ok = __all_sync(0xffffffffu,
+                        mbar_wait(&bar->s_full[j & 1], static_cast<uint32_t>(j >> 1) & 1u,
+                                  abort_flag, kDevWaitTimeoutSoftmax));
+        if (!ok) return;
+        tc_fence_after();
+        tmem_ld16(s_tmem, l1);
+        tmem_ld16(s_tmem + 16, l2);
+        note = bar->note[j % kNotes];
+      }
+      tmem_wait_ld();
+      after_wait(l1);
+      after_wait(l2);
+      tmem_ld16(s_tmem + 32, h1);
+      tmem_ld16(s_tmem + 48, h2);
+      const int valid = note.valid;
+      const float c = cq * note.k_scale;
       const uint64_t c2 = f2_pack(c, c);
+      const bool more = j + 1 < n_kv;
       uint64_t sum2[2] = {0ull, 0ull};
-      bool done = false, need_rescale = false, hi_pending = true;
-      float f = 1.0f;
-      if (valid == kKeys && __all_sync(0xffffffffu, m_ref != -INFINITY)) {
-        // Usual case: the reference stands, so the exponentials need not wait
-        // for the row max; if it moved past, the block is read again below.
-        const int mx =
-            exp_scores<TV, true, false, true>(v, c2, f2_pack(-m_ref, -m_ref), valid, sum2);
-        hi_pending = false;
-        done = !__any_sync(0xffffffffu, i2f_exact(mx) * c > m_ref + 8.0f);
-        if (!done) {
-          sum2[0] = sum2[1] = 0ull;
-          tmem_ld32(s_tmem, *reinterpret_cast<uint32_t(*)[32]>(v));
-          tmem_ld32(s_tmem + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
-          tmem_wait_ld();
+      bool done = false;
+      loaded = false;
+      if (__builtin_expect(primed && valid == kKeys, 1)) {
+        // The reference stands, so the exponentials need not wait for the row
+        // max; if it moved past, the block is read again below.
+        const uint64_t nm2 = f2_pack(-m_ref, -m_ref);
+        int mx = exp_scores<TV, true, false>(l1, l2, c2, nm2, valid, sum2);
+        tmem_wait_ld();
+        after_wait(h1);
+        after_wait(h2);
+        mx = max(mx, exp_scores<TV, true, false>(h1, h2, c2, nm2, valid, sum2));
+        // S(j + 1) was issued when P(j - 1) came: by now it is there, not before.
+        asm volatile("" : "+l"(sum2[0]), "+l"(sum2[1]));
+        const uint32_t next_s = static_cast<uint32_t>(j + 1) & 1u;
+        const bool ready = more && mbar_try_wait(smem_u32(&bar->s_full[next_s]),
+                                                 static_cast<uint32_t>((j + 1) >> 1) & 1u);
+        const uint32_t votes = __reduce_or_sync(
+            0xffffffffu,
+            (i2f_exact(mx) * c > m_ref + kGrowth<TV> ? 1u : 0u) | (ready ? 0u : 2u));
+        done = (votes & 1u) == 0u;
+        loaded = votes == 0u;
+        if (__builtin_expect(loaded, 1)) {
+          tc_fence_after();
+          tmem_ld16(s_tmem0 + next_s * kKeys, h2);
+          tmem_ld16(s_tmem0 + next_s * kKeys + 16, l2);
+          note = bar->note[(j + 1) % kNotes];
         }
       }
-      if (!done) {
-        if (hi_pending) tmem_wait_ld_regs(*reinterpret_cast<uint32_t(*)[32]>(v + 32));
+      if (__builtin_expect(!done, 0)) {
+        // The first block, a partly visible one, or one that moves the reference
+        // point of some row: the row max first.
+        tmem_wait_ld();
+        after_wait(h1);
+        after_wait(h2);
+        tmem_ld16(s_tmem, l1);
+        tmem_ld16(s_tmem + 16, l2);
+        tmem_ld16(s_tmem + 32, h1);
+        tmem_ld16(s_tmem + 48, h2);
+        tmem_wait_ld();
+        after_wait(l1);
+        after_wait(l2);
+        after_wait(h1);
+        after_wait(h2);
         int mx = INT32_MIN;
 #pragma unroll
-        for (int i = 0; i < kKeys; i += 2)
-          mx = __vimax3_s32(mx, i < valid ? static_cast<int>(v[i]) : INT32_MIN,
-                            i + 1 < valid ? static_cast<int>(v[i + 1]) : INT32_MIN);
+        for (int i = 0; i < kQuarter; ++i) {
+          mx = __vimax3_s32(mx, i < valid ? static_cast<int>(l1[i]) : INT32_MIN,
+                            i + 16 < valid ? static_cast<int>(l2[i]) : INT32_MIN);
+          mx = __vimax3_s32(mx, i + 32 < valid ? static_cast<int>(h1[i]) : INT32_MIN,
+                            i + 48 < valid ? static_cast<int>(h2[i]) : INT32_MIN);
+        }
         const float m_blk = i2f_exact(mx) * c;
-        const bool move = m_blk > m_ref + 8.0f;
+        const bool move = m_blk > m_ref + kGrowth<TV>;
         const bool rescale = move && m_ref != -INFINITY;
-        need_rescale = __any_sync(0xffffffffu, rescale);
-        f = rescale ? ex2(m_ref - m_blk) : 1.0f;
+        const float f = rescale ? ex2(m_ref - m_blk) : 1.0f;
         dsum *= f;
         if (move) m_ref = m_blk;
+        primed = __all_sync(0xffffffffu, m_ref != -INFINITY);
         const float nm = m_ref == -INFINITY ? 0.0f : -m_ref;
-        exp_scores<TV, false, true, false>(v, c2, f2_pack(nm, nm), valid, sum2);
-      }
-      tmem_st32(s_tmem, *reinterpret_cast<const uint32_t(*)[32]>(v));
-      const uint64_t s01 = f2_add(sum2[0], sum2[1]);
-      dsum += f2_lo(s01) + f2_hi(s01);
-      if (valid < kKeys && key_len < p.Lk) {
-        // V rows past key_lengths hold whatever the padding holds; a NaN there
-        // times p = 0 would still be NaN, so the rows are cleared.
-        ok = __all_sync(0xffffffffu,
-                        mbar_wait(&bar->kv_full[j % kStages],
-                                  static_cast<uint32_t>(j / kStages) & 1u, abort_flag,
-                                  kDevWaitTimeoutSoftmax));
-        if (!ok) break;
-        unsigned char* vt = kv_smem + (j % kStages) * kStageBytes + kKBytes;
-        for (int i = threadIdx.x; i < (kKeys - valid) * 16; i += kSoftmaxWarps * 32)
-          *reinterpret_cast<uint4*>(vt + (i & 8 ? kKeys * 128 : 0) + (valid + (i >> 4)) * 128 +
-                                    (i & 7) * 16) = make_uint4(0, 0, 0, 0);
-        fence_proxy_async_smem();
-      }
-      if (need_rescale) {
-        // O holds PV(0 .. j-1) once the commit after PV(j - 1) arrived; PV(j)
-        // waits for this warp's p_full arrival below.
-        const bool waited =
-            j + 1 < n_kv
-                ? mbar_wait(&bar->s_full[(j + 1) & 1], static_cast<uint32_t>((j + 1) >> 1) & 1u,
-                            abort_flag, kDevWaitTimeoutSoftmax)
-                : mbar_wait(&bar->o_done, 0u, abort_flag, kDevWaitTimeoutSoftmax);
-        ok = __all_sync(0xffffffffu, waited);
-        if (!ok) break;
-        tc_fence_after();
+        sum2[0] = sum2[1] = 0ull;
+        exp_scores<TV, false, true>(l1, l2, c2, f2_pack(nm, nm), valid, sum2);
+        exp_scores<TV, false, true>(h1, h2, c2, f2_pack(nm, nm), valid - 32, sum2);
+        if (valid < kKeys && key_len < p.Lk) {
+          // V rows past key_lengths hold whatever the padding holds; a NaN there
+          // times p = 0 would still be NaN, so the rows are cleared.
+          ok = __all_sync(0xffffffffu,
+                          mbar_wait(&bar->v_full[j % kStages],
+                                    static_cast<uint32_t>(j / kStages) & 1u, abort_flag,
+                                    kDevWaitTimeoutSoftmax));
+          if (!ok) return;
+          unsigned char* vt = v_smem + (j % kStages) * kVBytes;
+          for (int i = threadIdx.x; i < (kKeys - valid) * 16; i += kSoftmaxWarps * 32)
+            *reinterpret_cast<uint4*>(vt + (i & 8 ? kKeys * 128 : 0) + (valid + (i >> 4)) * 128 +
+                                      (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+          fence_proxy_async_smem();
+        }
+        if (__any_sync(0xffffffffu, rescale)) {
+          // O holds PV(0 .. j-1) once the commit after PV(j - 1) arrived; PV(j)
+          // waits for this warp's p_full arrival below.
+          const bool waited =
+              more
+                  ? mbar_wait(&bar->s_full[(j + 1) & 1], static_cast<uint32_t>((j + 1) >> 1) & 1u,
+                              abort_flag, kDevWaitTimeoutSoftmax)
+                  : mbar_wait(&bar->o_done, 0u, abort_flag, kDevWaitTimeoutSoftmax);
+          ok = __all_sync(0xffffffffu, waited);
+          if (!ok) return;
+          tc_fence_after();
 #pragma unroll 1
-        for (int cc = 0; cc < kDim / 16; ++cc) {
-          uint32_t o[16];
-          tmem_ld16(o_tmem + cc * 16, o);
-          tmem_wait_ld();
+          for (int cc = 0; cc < kDim / 16; ++cc) {
+            uint32_t o[16];
+            tmem_ld16(o_tmem + cc * 16, o);
+            tmem_wait_ld();
+            after_wait(o);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-          tmem_st16(o_tmem + cc * 16, o);
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_st16(o_tmem + cc * 16, o);
+          }
         }
       }
+      tmem_st16(s_tmem, l1);
+      tmem_st16(s_tmem + 16, h1);
+      const uint64_t s01 = f2_add(sum2[0], sum2[1]);
+      dsum += f2_lo(s01) + f2_hi(s01);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar->p_full[j & 1]);
+    };
+    uint32_t r0[kQuarter], r1[kQuarter], r2[kQuarter], r3[kQuarter];
+    for (int j = 0; j < n_kv && ok; j += 2) {
+      block(j, r0, r1, r2, r3);
+      if (ok && j + 1 < n_kv) block(j + 1, r3, r1, r2, r0);
     }
     if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&bar->o_final, 0u, abort_flag,
                                                    kDevWaitTimeoutSoftmax));
@@ -438,20 +530,23 @@ __global__ void __launch_bounds__(kThreads, 2)
           tmem_ld16(o_tmem + cc * 16, o);
           tmem_wait_ld();
         }
-        if (row >= p.Lq) continue;
-        if (prow != nullptr) {
+        if (row < p.Lq) {
+          if (prow != nullptr) {
 #pragma unroll
-          for (int i = 0; i < 16; i += 4)
-            *reinterpret_cast<uint4*>(prow + cc * 16 + i) =
-                make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-        } else {
-          uint32_t w[8];
+            for (int i = 0; i < 16; i += 4)
+              *reinterpret_cast<uint4*>(prow + cc * 16 + i) =
+                  make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          } else {
+            uint32_t w[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            w[i] = pack2<TV>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
-          *reinterpret_cast<uint4*>(orow + cc * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-          *reinterpret_cast<uint4*>(orow + cc * 16 + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+            for (int i = 0; i < 8; ++i)
+              w[i] =
+                  pack2<TV>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+            *reinterpret_cast<uint4*>(orow + cc * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(orow + cc * 16 + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+          }
         }
+        __syncwarp();
       }
       if (row < p.Lq) {
         if (p.splits > 1) p.part_md[flat * p.splits + split] = make_float2(m_ref, dsum);
