@@ -138,26 +138,31 @@ struct ListCursor {
 template <typename TV>
 __device__ constexpr float kGrowth = std::is_same<TV, __nv_bfloat16>::value ? 32.0f : 12.0f;
 
-// p = 2^(s c - m) of 32 scores of a block, 16 in x and 16 in y; the packed pairs
-// of V's type replace x, y is free.  `sum2` gathers the unrounded p.  Returns
-// the integer row max where TRACK_MAX.  MASKED zeroes keys >= valid.
-template <typename TV, bool TRACK_MAX, bool MASKED>
-__device__ __forceinline__ int exp_scores(uint32_t (&x)[kQuarter], uint32_t (&y)[kQuarter],
-                                          uint64_t c2, uint64_t nm2, int valid,
-                                          uint64_t (&sum2)[2]) {
-  int m[2] = {INT32_MIN, INT32_MIN};
+// p = 2^(s c - m) of the 16 scores in x; the packed pairs of V's type go to
+// out[AT .. AT + 7] (which may be x's own first half).  `sum2` gathers the
+// unrounded p.  MASKED zeroes keys >= valid.
+template <typename TV, int AT, bool MASKED>
+__device__ __forceinline__ void exp_scores(uint32_t (&x)[kQuarter], uint32_t (&out)[kQuarter],
+                                           uint64_t c2, uint64_t nm2, int valid,
+                                           uint64_t (&sum2)[2]) {
 #pragma unroll
-  for (int i = 0; i < kQuarter; ++i) {
-    const uint32_t s0 = i < kQuarter / 2 ? x[2 * i] : y[2 * i - kQuarter];
-    const uint32_t s1 = i < kQuarter / 2 ? x[2 * i + 1] : y[2 * i + 1 - kQuarter];
-    if (TRACK_MAX) m[i & 1] = __vimax3_s32(m[i & 1], static_cast<int>(s0), static_cast<int>(s1));
-    uint64_t p2 = ex2_pair(f2_fma(score_pair_f32(s0, s1), c2, nm2));
+  for (int i = 0; i < kQuarter / 2; ++i) {
+    uint64_t p2 = ex2_pair(f2_fma(score_pair_f32(x[2 * i], x[2 * i + 1]), c2, nm2));
     if (MASKED)
       p2 = f2_pack(2 * i < valid ? f2_lo(p2) : 0.0f, 2 * i + 1 < valid ? f2_hi(p2) : 0.0f);
     sum2[i & 1] = f2_add(sum2[i & 1], p2);
-    x[i] = pack_pair<TV>(p2);
+    out[AT + i] = pack_pair<TV>(p2);
   }
-  return max(m[0], m[1]);
+}
+
+__device__ __forceinline__ int max_score(const uint32_t (&x)[kQuarter], int m) {
+  int m2 = INT32_MIN;
+#pragma unroll
+  for (int i = 0; i < kQuarter; i += 4) {
+    m = __vimax3_s32(m, static_cast<int>(x[i]), static_cast<int>(x[i + 1]));
+    m2 = __vimax3_s32(m2, static_cast<int>(x[i + 2]), static_cast<int>(x[i + 3]));
+  }
+  return max(m, m2);
 }
 
 // Keeps uses of loaded registers behind the tmem_wait_ld before it.
@@ -405,21 +410,24 @@ __global__ void __launch_bounds__(kThreads, 2)
         // The reference stands, so the exponentials need not wait for the row
         // max; if it moved past, the block is read again below.
         const uint64_t nm2 = f2_pack(-m_ref, -m_ref);
-        int mx = exp_scores<TV, true, false>(l1, l2, c2, nm2, valid, sum2);
+        const int mx_low = max_score(l2, max_score(l1, INT32_MIN));
+        exp_scores<TV, 0, false>(l1, l1, c2, nm2, kKeys, sum2);
+        exp_scores<TV, 8, false>(l2, l1, c2, nm2, kKeys, sum2);
         tmem_wait_ld();
         after_wait(h1);
         after_wait(h2);
-        mx = max(mx, exp_scores<TV, true, false>(h1, h2, c2, nm2, valid, sum2));
-        // S(j + 1) was issued when P(j - 1) came: by now it is there, not before.
-        asm volatile("" : "+l"(sum2[0]), "+l"(sum2[1]));
+        // Both votes are taken under exponentials that do not wait for them.
+        const int mx = max_score(h2, max_score(h1, mx_low));
+        const bool past = __any_sync(0xffffffffu, i2f_exact(mx) * c > m_ref + kGrowth<TV>);
+        exp_scores<TV, 0, false>(h1, h1, c2, nm2, kKeys, sum2);
+        // S(j + 1) was issued when P(j - 1) came: not sooner than here is it there.
+        asm volatile("" : "+l"(sum2[0]));
         const uint32_t next_s = static_cast<uint32_t>(j + 1) & 1u;
-        const bool ready = more && mbar_try_wait(smem_u32(&bar->s_full[next_s]),
-                                                 static_cast<uint32_t>((j + 1) >> 1) & 1u);
-        const uint32_t votes = __reduce_or_sync(
-            0xffffffffu,
-            (i2f_exact(mx) * c > m_ref + kGrowth<TV> ? 1u : 0u) | (ready ? 0u : 2u));
-        done = (votes & 1u) == 0u;
-        loaded = votes == 0u;
+        const bool ready = mbar_try_wait(smem_u32(&bar->s_full[next_s]),
+                                         static_cast<uint32_t>((j + 1) >> 1) & 1u);
+        exp_scores<TV, 8, false>(h2, h1, c2, nm2, kKeys, sum2);
+        done = !past;
+        loaded = done && more && __all_sync(0xffffffffu, ready);
         if (__builtin_expect(loaded, 1)) {
           tc_fence_after();
           tmem_ld16(s_tmem0 + next_s * kKeys, h2);
@@ -459,8 +467,10 @@ __global__ void __launch_bounds__(kThreads, 2)
         primed = __all_sync(0xffffffffu, m_ref != -INFINITY);
         const float nm = m_ref == -INFINITY ? 0.0f : -m_ref;
         sum2[0] = sum2[1] = 0ull;
-        exp_scores<TV, false, true>(l1, l2, c2, f2_pack(nm, nm), valid, sum2);
-        exp_scores<TV, false, true>(h1, h2, c2, f2_pack(nm, nm), valid - 32, sum2);
+        exp_scores<TV, 0, true>(l1, l1, c2, f2_pack(nm, nm), valid, sum2);
+        exp_scores<TV, 8, true>(l2, l1, c2, f2_pack(nm, nm), valid - 16, sum2);
+        exp_scores<TV, 0, true>(h1, h1, c2, f2_pack(nm, nm), valid - 32, sum2);
+        exp_scores<TV, 8, true>(h2, h1, c2, f2_pack(nm, nm), valid - 48, sum2);
         if (valid < kKeys && key_len < p.Lk) {
           // V rows past key_lengths hold whatever the padding holds; a NaN there
           // times p = 0 would still be NaN, so the rows are cleared.
