@@ -79,7 +79,8 @@ struct SelectParams {
   int query_blocks, key_blocks, keep, policy_rows;
   int q_tiles_scale;
   int rows_cta;                // query blocks per CTA, <= kMaxRows
-  int groups;                  // CTAs per key head
+  int groups;                  // row groups per key head
+  int cluster;                 // CTAs that share a row group's key blocks
   float z, slope;              // normal quantile that `keep` of the key blocks exceed; deviations
                                // that one block more or less moves it there
   int8_t* q_digits;            // [B * Hq * query_blocks, kQDigits, kChannels]
@@ -505,6 +506,9 @@ __device__ __forceinline__ bool choose_row(const uint32_t* row, int n, int keep,
   return true;
 }
 
+__device__ __forceinline__ void store_cluster(uint32_t cluster_addr, uint32_t value) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(value) : "memory");
+}
 __device__ __forceinline__ int64_t mad_wide(int a, int b, int c) {
   int64_t d;
   asm("mad.wide.s32 %0, %1, %2, %3;" : "=l"(d) : "r"(a), "r"(b), "l"(static_cast<int64_t>(c)));
@@ -526,15 +530,19 @@ __global__ void __launch_bounds__(kSelectThreads, 2)
   uint32_t* keys = reinterpret_cast<uint32_t*>(bar + 1);  // [rows][row_keys], zeros past `blocks`
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t kv = blockIdx.x / p.groups;               // (batch, key head)
+  const int rank = static_cast<int>(blockIdx.x) % p.cluster;
+  const int group = static_cast<int>(blockIdx.x) / p.cluster;
+  const int64_t kv = group / p.groups;                    // (batch, key head)
   const int b = static_cast<int>(kv / p.Hk);
   const int head_rows = p.Hq / p.Hk * p.query_blocks;     // query blocks of the key head
-  const int row_in_head = (blockIdx.x % p.groups) * p.rows_cta;
+  const int row_in_head = (group % p.groups) * p.rows_cta;
   const int rows = min(p.rows_cta, head_rows - row_in_head);
   const int64_t row0 = kv * head_rows + row_in_head;
   const int key_len = visible_keys(p, b);
   const int blocks = (key_len + kKeyBlock - 1) / kKeyBlock;
-  int tiles = (blocks + kTileKeys - 1) / kTileKeys;
+  // This CTA takes every cluster-th tile from its rank on.
+  const int all_tiles = (blocks + kTileKeys - 1) / kTileKeys;
+  int tiles = (all_tiles - rank + p.cluster - 1) / p.cluster;
   const int row_keys = 32 * keys_per_lane(blocks);
 
   if (threadIdx.x == 0) {
@@ -563,6 +571,7 @@ __global__ void __launch_bounds__(kSelectThreads, 2)
   }
   tc_fence_before();
   __syncthreads();
+  if (p.cluster > 1) cluster_sync_all();  // rank 0 has started: its keys can be written
   tc_fence_after();
   const uint32_t tmem = bar->tmem_base;
   volatile int* abort_flag = &bar->abort_flag;
@@ -581,7 +590,8 @@ __global__ void __launch_bounds__(kSelectThreads, 2)
                        abort_flag, kDevWaitTimeoutProducer))
           break;
         mbar_arrive_expect_tx(&bar->full[s], kStageBytes);
-        tma_load_4d(ring + s * kStageBytes, &tm_k, &bar->full[s], 0, issued / kKDigits * kTileKeys,
+        tma_load_4d(ring + s * kStageBytes, &tm_k, &bar->full[s], 0,
+                    (issued / kKDigits * p.cluster + rank) * kTileKeys,
                     static_cast<int>(kv), issued % kKDigits);
       }
       // Every copy lands before the CTA exits.
@@ -620,11 +630,14 @@ __global__ void __launch_bounds__(kSelectThreads, 2)
     // Warps 0-3 take the even tiles, 4-7 the odd ones: one key block per thread.
     const int buf = warp >> 2, quad = warp & 3;
     const double* factors = p.k_factor + kv * p.key_blocks;
-    int j = buf * kTileKeys + quad * 32 + lane;
+    const int stride = 2 * p.cluster * kTileKeys;  // to this warp's next tile
+    int j = (buf * p.cluster + rank) * kTileKeys + quad * 32 + lane;
     double next_factor = j < blocks ? factors[j] : 0.0;
-    for (int t = buf; t < tiles; t += 2, j += 2 * kTileKeys) {
+    // Rank 0 keeps the keys.
+    const uint32_t keys_at = p.cluster > 1 ? mapa_shared(smem_u32(keys), 0u) : 0u;
+    for (int t = buf; t < tiles; t += 2, j += stride) {
       const double factor = next_factor;
-      if (j + 2 * kTileKeys < blocks) next_factor = factors[j + 2 * kTileKeys];
+      if (j + stride < blocks) next_factor = factors[j + stride];
       if (!__all_sync(0xffffffffu,
                       mbar_wait(&bar->tmem_full[buf], static_cast<uint32_t>(t >> 1) & 1u,
                                 abort_flag, kDevWaitTimeoutEpilogue)))
@@ -646,7 +659,6 @@ __global__ void __launch_bounds__(kSelectThreads, 2)
           after_wait(lo[d]);
           after_wait(hi[d]);
         }
-        uint32_t* dst = keys + r0 * row_keys + j;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           // Digit sums of weight 128^w, two to a 32-bit integer, four to an int64.
@@ -658,14 +670,23 @@ __global__ void __launch_bounds__(kSelectThreads, 2)
           const uint32_t key =
               top_word(exact_score(low + static_cast<int64_t>(static_cast<uint64_t>(high) << 28),
                                    factor));
-          if (j < blocks && r0 + i < rows) dst[i * row_keys] = key;
+          if (j < blocks && r0 + i < rows) {
+            const int at = (r0 + i) * row_keys + j;
+            if (p.cluster > 1) store_cluster(keys_at + 4u * static_cast<uint32_t>(at), key);
+            else keys[at] = key;
+          }
         }
       }
       if (p.policy != nullptr && j < blocks) {
         for (int r = 0; r < rows; ++r) {
           const int prow = p.policy_rows == 1 ? 0 : (row_in_head + r) % p.query_blocks;
           const int pol = p.policy[static_cast<int64_t>(prow) * p.key_blocks + j];
-          if (pol != 0) keys[r * row_keys + j] = pol < 0 ? 0u : ~0u;
+          if (pol != 0) {
+            const int at = r * row_keys + j;
+            const uint32_t key = pol < 0 ? 0u : ~0u;
+            if (p.cluster > 1) store_cluster(keys_at + 4u * static_cast<uint32_t>(at), key);
+            else keys[at] = key;
+          }
         }
       }
       tc_fence_before();
@@ -679,7 +700,8 @@ __global__ void __launch_bounds__(kSelectThreads, 2)
     tc_fence_after();
     tmem_dealloc(tmem, kTmemCols);
   }
-  if (warp >= rows || *abort_flag) return;
+  if (p.cluster > 1) cluster_sync_all();  // every tile's keys are in rank 0's memory
+  if (rank != 0 || warp >= rows || *abort_flag) return;
 
   uint32_t* row = keys + warp * row_keys;
   const int64_t grow = row0 + warp;
@@ -765,6 +787,14 @@ void select_launch(SelectParams& p, cudaStream_t stream) {
           heads * ((head_rows + p.rows_cta - 1) / p.rows_cta) < device_sm_count()))
     p.rows_cta /= 2;
   p.groups = static_cast<int>((head_rows + p.rows_cta - 1) / p.rows_cta);
+  // Few row groups (single tokens): a cluster shares each one's key blocks, as
+  // many CTAs as fill two per SM with at least two tiles each (one token, 32 heads,
+  // 2048 key blocks: 30 us alone, 11 with clusters of 8).
+  const int64_t tiles = (p.key_blocks + kTileKeys - 1) / kTileKeys;
+  p.cluster = 1;
+  while (p.cluster < 8 && 2 * p.cluster * heads * p.groups <= 2 * device_sm_count() &&
+         4 * p.cluster <= tiles)
+    p.cluster *= 2;
   CUtensorMap tq, tk;
   {
     const uint64_t dims[3] = {kChannels, kQDigits, static_cast<uint64_t>(heads * head_rows)};
@@ -785,8 +815,19 @@ void select_launch(SelectParams& p, cudaStream_t stream) {
   auto launch = [&](auto kern) {
     TB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        static_cast<int>(smem)));
-    kern<<<static_cast<unsigned>(heads * p.groups), kSelectThreads, smem, stream>>>(tq, tk, p);
-    TB_CUDA_CHECK(cudaGetLastError());
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(heads * p.groups * p.cluster));
+    cfg.blockDim = dim3(kSelectThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = static_cast<unsigned>(p.cluster);
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    TB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, tq, tk, p));
   };
   // As many register keys as a row needs; past 41 a lane the kernel would spill
   // and the rest of a row is read from shared memory.

@@ -240,8 +240,8 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeParams p) 
 // thread of G pairs writes 4 G values at once.
 template <typename T, int G>
 __global__ void __launch_bounds__(kRopeThreads)
-    rope_freqs_kernel(const RopePositions pos, T* __restrict__ out, int batch, int length,
-                      int pairs, int groups_cta, int tok_lanes) {
+    rope_freqs_kernel(const RopePositions pos, T* __restrict__ out, int length, int pairs,
+                      int groups_cta, int tok_lanes) {
   const int g = blockIdx.y * groups_cta + threadIdx.x % groups_cta;
   const int lane = threadIdx.x / groups_cta;
   if (g * G >= pairs || lane >= tok_lanes) return;
@@ -252,11 +252,11 @@ __global__ void __launch_bounds__(kRopeThreads)
     f[i] = pos.inv_freq[g * G + i];
     axis[i] = axis_of(pos, g * G + i);
   }
-  const int64_t tokens = static_cast<int64_t>(batch) * length;
-  for (int64_t t = static_cast<int64_t>(blockIdx.x) * tok_lanes + lane; t < tokens;
-       t += static_cast<int64_t>(gridDim.x) * tok_lanes) {
-    const int b = static_cast<int>(t / length);
-    const int64_t at = b * pos.batch_stride + (t - static_cast<int64_t>(b) * length) * pos.axes;
+  const int64_t b = blockIdx.z;
+  const int step = static_cast<int>(gridDim.x) * tok_lanes;
+#pragma unroll 2
+  for (int t = static_cast<int>(blockIdx.x) * tok_lanes + lane; t < length; t += step) {
+    const int64_t at = b * pos.batch_stride + static_cast<int64_t>(t) * pos.axes;
     float v[4 * G];
 #pragma unroll
     for (int i = 0; i < G; ++i) {
@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(kRopeThreads)
       v[4 * i + 2] = s;
       v[4 * i + 3] = c;
     }
-    T* o = out + (t * pairs + g * G) * 4;
+    T* o = out + ((b * length + t) * pairs + g * G) * 4;
     if constexpr (sizeof(T) == 4) {
       *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
     } else {
@@ -365,20 +365,24 @@ void freqs_launch(const RopePositions& pos, void* out, int64_t batch, int64_t le
   const int groups = two ? pairs / 2 : pairs;
   const int groups_cta = std::min(groups, kRopeThreads);
   const int tok_lanes = kRopeThreads / groups_cta;
-  const int64_t blocks = (batch * length + tok_lanes - 1) / tok_lanes;
-  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks, 16LL * device_sm_count())),
-                  static_cast<unsigned>((groups + groups_cta - 1) / groups_cta));
+  // Eight CTAs fit an SM; a few tokens per thread share its frequencies.
+  const int64_t blocks = (length + tok_lanes - 1) / tok_lanes;
+  const int64_t want = std::max<int64_t>(1, 16LL * device_sm_count() / batch);
+  TB_REQUIRE(batch <= 65535, "batch exceeds the grid range");
+  const dim3 grid(static_cast<unsigned>(std::min(blocks, want)),
+                  static_cast<unsigned>((groups + groups_cta - 1) / groups_cta),
+                  static_cast<unsigned>(batch));
   T* o = static_cast<T*>(out);
-  const int B = static_cast<int>(batch), L = static_cast<int>(length);
+  const int L = static_cast<int>(length);
   if constexpr (sizeof(T) == 2) {
     if (two) {
-      rope_freqs_kernel<T, 2><<<grid, kRopeThreads, 0, stream>>>(pos, o, B, L, pairs, groups_cta,
+      rope_freqs_kernel<T, 2><<<grid, kRopeThreads, 0, stream>>>(pos, o, L, pairs, groups_cta,
                                                                   tok_lanes);
       TB_CUDA_CHECK(cudaGetLastError());
       return;
     }
   }
-  rope_freqs_kernel<T, 1><<<grid, kRopeThreads, 0, stream>>>(pos, o, B, L, pairs, groups_cta,
+  rope_freqs_kernel<T, 1><<<grid, kRopeThreads, 0, stream>>>(pos, o, L, pairs, groups_cta,
                                                              tok_lanes);
   TB_CUDA_CHECK(cudaGetLastError());
 }
@@ -443,7 +447,7 @@ extern "C" int tb_rope_freqs(const void* positions, int position_type, int64_t p
     TB_REQUIRE(dtype == TB_DTYPE_BF16 || dtype == TB_DTYPE_F16 || dtype == TB_DTYPE_F32,
                "rotary matrices must be float16, bfloat16, or float32");
     TB_REQUIRE(batch > 0 && length > 0 && pairs > 0, "rotary input dimensions must be positive");
-    TB_REQUIRE(pairs <= 32768 && length <= INT32_MAX && batch <= INT32_MAX,
+    TB_REQUIRE(pairs <= 32768 && length <= INT32_MAX / 2 && batch <= INT32_MAX,
                "rotary dimensions exceed the CUDA kernel range");
     TB_REQUIRE((reinterpret_cast<uintptr_t>(output) & 15u) == 0,
                "rotary matrices must be 16-byte aligned");

@@ -575,7 +575,9 @@ __global__ void __launch_bounds__(kThreads, 2)
 }
 
 // Joins the partial results of a split list: one warp per row, four channels
-// per lane; O = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) d_s.
+// per lane; O = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) d_s.  Lane s holds the
+// m and d of part s (32 at a time), so the loads of one row do not wait for one
+// another.
 template <typename TV>
 __global__ void __launch_bounds__(kCombineWarps * 32) sparse_combine_kernel(const SparseParams p,
                                                                             int64_t rows) {
@@ -583,23 +585,34 @@ __global__ void __launch_bounds__(kCombineWarps * 32) sparse_combine_kernel(cons
   const int lane = threadIdx.x & 31;
   if (flat >= rows) return;
   const float2* md = p.part_md + flat * p.splits;
+  const float* part = p.part_o + flat * p.splits * kDim + lane * 4;
   float M = -INFINITY;
-  for (int s = 0; s < p.splits; ++s)
-    if (md[s].y != 0.0f) M = fmaxf(M, md[s].x);
+  for (int s = lane; s < p.splits; s += 32) {
+    const float2 t = md[s];
+    if (t.y != 0.0f) M = fmaxf(M, t.x);
+  }
+#pragma unroll
+  for (int m = 16; m > 0; m >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, m));
   float d = 0.0f;
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int s = 0; s < p.splits; ++s) {
-    const float2 t = md[s];
-    if (t.y == 0.0f) continue;  // saw no key
-    // m = -inf with d != 0: every score of the part was NaN.
-    const float w = t.x == -INFINITY ? 1.0f : ex2(t.x - M);
-    const float4 q =
-        *reinterpret_cast<const float4*>(p.part_o + (flat * p.splits + s) * kDim + lane * 4);
-    d = fmaf(w, t.y, d);
-    o.x = fmaf(w, q.x, o.x);
-    o.y = fmaf(w, q.y, o.y);
-    o.z = fmaf(w, q.z, o.z);
-    o.w = fmaf(w, q.w, o.w);
+  for (int s0 = 0; s0 < p.splits; s0 += 32) {
+    const int n = min(32, p.splits - s0);
+    const float2 mine = lane < n ? md[s0 + lane] : make_float2(0.0f, 0.0f);
+    // d = 0: saw no key.  m = -inf with d != 0: every score of the part was NaN.
+    const float w = mine.y == 0.0f ? 0.0f : (mine.x == -INFINITY ? 1.0f : ex2(mine.x - M));
+#pragma unroll 8
+    for (int s = 0; s < n; ++s) {
+      const float ws = __shfl_sync(0xffffffffu, w, s);
+      const float ds = __shfl_sync(0xffffffffu, mine.y, s);
+      const float4 q = *reinterpret_cast<const float4*>(part + (s0 + s) * kDim);
+      if (ds != 0.0f) {
+        d = fmaf(ws, ds, d);
+        o.x = fmaf(ws, q.x, o.x);
+        o.y = fmaf(ws, q.y, o.y);
+        o.z = fmaf(ws, q.z, o.z);
+        o.w = fmaf(ws, q.w, o.w);
+      }
+    }
   }
   const float inv = d > 0.0f ? 1.0f / d : (d == 0.0f ? 0.0f : d);
   const int bh = static_cast<int>(flat / p.Lq);
