@@ -789,7 +789,7 @@ void select_launch(SelectParams& p, cudaStream_t stream) {
   p.groups = static_cast<int>((head_rows + p.rows_cta - 1) / p.rows_cta);
   // Few row groups (single tokens): a cluster shares each one's key blocks, as
   // many CTAs as fill two per SM with at least two tiles each (one token, 32 heads,
-  // 2048 key blocks: 30 us alone, 11 with clusters of 8).
+  // 2048 key blocks: 30 us alone, 18 with clusters of 8).
   const int64_t tiles = (p.key_blocks + kTileKeys - 1) / kTileKeys;
   p.cluster = 1;
   while (p.cluster < 8 && 2 * p.cluster * heads * p.groups <= 2 * device_sm_count() &&
@@ -829,8 +829,9 @@ void select_launch(SelectParams& p, cudaStream_t stream) {
     cfg.numAttrs = 1;
     TB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, tq, tk, p));
   };
-  // As many register keys as a row needs; past 41 a lane the kernel would spill
-  // and the rest of a row is read from shared memory.
+  // As many register keys as a row needs; past 41 a lane (1312 key blocks) the
+  // rest of a row is read from shared memory: 81 in registers cost the second CTA
+  // of an SM (one token, 2048 key blocks: 22 against 18 us).
   const int per_lane = keys_per_lane(p.key_blocks);
   if (per_lane <= 9) launch(block_select_kernel<9>);
   else if (per_lane <= 17) launch(block_select_kernel<17>);

@@ -31,7 +31,7 @@ namespace {
 constexpr int kRopeThreads = 256;
 constexpr int kRopeInFlight = 4;
 constexpr int kMaxAxes = 4;
-constexpr double kInvTwoPi = 0.15915494309189535;
+constexpr double kTwoOverPi = 0.6366197723675814;
 
 struct RopePositions {
   const void* ptr;
@@ -59,7 +59,12 @@ struct RopeParams {
 __device__ __forceinline__ double load_position(const RopePositions& p, int64_t i) {
   switch (p.type) {
     case TB_POS_I32: return static_cast<double>(static_cast<const int32_t*>(p.ptr)[i]);
-    case TB_POS_I64: return static_cast<double>(static_cast<const int64_t*>(p.ptr)[i]);
+    case TB_POS_I64: {
+      // Exact up to 2^51 by the mantissa of 1.5 * 2^52 (64-bit conversions are slow;
+      // larger positions have no phase left in fp64).
+      const int64_t v = static_cast<const int64_t*>(p.ptr)[i];
+      return __longlong_as_double(v + 0x4338000000000000ll) - 6755399441055744.0;
+    }
     case TB_POS_F32: return static_cast<double>(static_cast<const float*>(p.ptr)[i]);
     default: return static_cast<const double*>(p.ptr)[i];
   }
@@ -72,12 +77,29 @@ __device__ __forceinline__ int axis_of(const RopePositions& p, int pair) {
   return a;
 }
 
-// scale * cos and scale * sin of position * inv_freq.
+// scale * cos and scale * sin of position * inv_freq.  In fp64 the angle is
+// counted in quarter turns and split into the nearest whole number (the low bits
+// of its sum with 1.5 * 2^52) and a rest r in [-1/2, 1/2]; sin and cos of r
+// quarter turns are polynomials in r^2 (interpolated at the Chebyshev nodes of
+// [0, 1/4]; off by at most 1 ulp with fp32 arithmetic), turned by the quadrant.
 __device__ __forceinline__ void turn(const RopePositions& p, double position, double inv_freq,
                                      float& c, float& s) {
-  const double turns = position * inv_freq * kInvTwoPi;
-  const float f = static_cast<float>(2.0 * (turns - rint(turns)));  // half turns in [-1, 1]
-  sincospif(f, &s, &c);
+  const double quarters = position * inv_freq * kTwoOverPi;
+  const double shifted = quarters + 6755399441055744.0;
+  const int q = __double2loint(shifted);
+  const float r = static_cast<float>(quarters - (shifted - 6755399441055744.0));
+  const float z = r * r;
+  float a = fmaf(z, -0.004602149128913879f, 0.07968021929264069f);
+  a = fmaf(z, a, -0.6459634900093079f);
+  a = fmaf(z, a, -4.371138828673793e-08f);  // pi / 2 in two words
+  a = fmaf(r, 1.5707963705062866f, r * a);
+  float b = fmaf(z, 0.0009067399078048766f, -0.02086152881383896f);
+  b = fmaf(z, b, 0.253669410943985f);
+  b = fmaf(z, b, -1.2337005138397217f);
+  b = fmaf(z, b, 1.0f);
+  const float sn = q & 1 ? b : a, cs = q & 1 ? a : b;
+  s = __uint_as_float(__float_as_uint(sn) ^ (static_cast<uint32_t>(q & 2) << 30));
+  c = __uint_as_float(__float_as_uint(cs) ^ (static_cast<uint32_t>((q + 1) & 2) << 30));
   c = fmaf(c, p.scale, c * p.scale_lo);
   s = fmaf(s, p.scale, s * p.scale_lo);
 }
@@ -258,10 +280,12 @@ __global__ void __launch_bounds__(kRopeThreads)
   for (int t = static_cast<int>(blockIdx.x) * tok_lanes + lane; t < length; t += step) {
     const int64_t at = b * pos.batch_stride + static_cast<int64_t>(t) * pos.axes;
     float v[4 * G];
+    double position = load_position(pos, at + axis[0]);
 #pragma unroll
     for (int i = 0; i < G; ++i) {
       float c, s;
-      turn(pos, load_position(pos, at + axis[i]), f[i], c, s);
+      if (i > 0 && axis[i] != axis[i - 1]) position = load_position(pos, at + axis[i]);
+      turn(pos, position, f[i], c, s);
       v[4 * i] = c;
       v[4 * i + 1] = -s;
       v[4 * i + 2] = s;
