@@ -352,7 +352,7 @@ __host__ __device__ constexpr int keys_per_lane(int n) { return ((n + 31) / 32) 
 // twice counts half); after 12 steps the middle key, which needs at most 32
 // more.  About 6 thresholds a row; halving the key range took 22.
 template <int PER_LANE>
-__device__ __forceinline__ bool choose_row(const uint32_t* row, int n, int keep, float z,
+__device__ __forceinline__ bool choose_row(uint32_t* row, int n, int keep, float z,
                                            float slope, bool settle, int32_t* out,
                                            uint32_t& edge) {
   const int lane = static_cast<int>(lane_id());
@@ -487,11 +487,19 @@ __device__ __forceinline__ bool choose_row(const uint32_t* row, int n, int keep,
   }
   const int total = __shfl_sync(0xffffffffu, at, 31);
   at -= mine;
-  if (exact) {
+  if (exact && per <= PER_LANE) {
+    // The keys are in registers: their places gather in the row's memory and
+    // leave it side by side.
 #pragma unroll
-    for (int i = 0; i < PER_LANE; ++i)
-      if (own[i] >= edge) out[at++] = first + i;
-    for (int i = PER_LANE; i < per; ++i)
+    for (int i = 0; i < PER_LANE; ++i) {
+      const bool take = own[i] >= edge;
+      if (take) row[at] = static_cast<uint32_t>(first + i);
+      at += take ? 1 : 0;
+    }
+    __syncwarp();
+    for (int j = lane; j < total; j += 32) out[j] = static_cast<int32_t>(row[j]);
+  } else if (exact) {
+    for (int i = 0; i < per; ++i)
       if (row[first + i] >= edge) out[at++] = first + i;
   } else {
     for (int i = 0; i < per; ++i) {
@@ -600,17 +608,20 @@ __global__ void __launch_bounds__(kSelectThreads, 2)
         drain_wait(&bar->full[i % kStages], static_cast<uint32_t>(i / kStages) & 1u);
     }
   } else if (warp == kMmaWarp) {
-    if (lane == 0 && tiles > 0) {
+    if (tiles > 0) {
       constexpr uint32_t idesc = idesc_i8(kTileKeys, kMmaN);
+      const uint32_t elected = elect_one();
       const uint64_t q_desc = umma_desc_sw128(smem_u32(smem));
-      bool ok = mbar_wait(&bar->q_full, 0, abort_flag, kDevWaitTimeoutMma);
+      auto warp_wait = [&](uint64_t* bar_, int phase) {
+        return __all_sync(0xffffffffu, mbar_wait(bar_, static_cast<uint32_t>(phase) & 1u,
+                                                 abort_flag, kDevWaitTimeoutMma)) != 0;
+      };
+      bool ok = warp_wait(&bar->q_full, 0);
       for (int t = 0; t < tiles && ok; ++t) {
-        ok = mbar_wait(&bar->tmem_empty[t & 1], (static_cast<uint32_t>(t >> 1) & 1u) ^ 1u,
-                       abort_flag, kDevWaitTimeoutMma);
+        ok = warp_wait(&bar->tmem_empty[t & 1], (t >> 1) + 1);
         for (int d = 0; d < kKDigits && ok; ++d) {
           const int i = t * kKDigits + d, s = i % kStages;
-          ok = mbar_wait(&bar->full[s], static_cast<uint32_t>(i / kStages) & 1u, abort_flag,
-                         kDevWaitTimeoutMma);
+          ok = warp_wait(&bar->full[s], i / kStages);
           if (!ok) break;
           tc_fence_after();
           const uint64_t k_desc = umma_desc_sw128(smem_u32(ring) + s * kStageBytes);
@@ -618,13 +629,15 @@ __global__ void __launch_bounds__(kSelectThreads, 2)
                                   static_cast<uint32_t>(d * kMmaN);
 #pragma unroll
           for (int kk = 0; kk < kChannels / 32; ++kk)
-            mma_i8_ss(d_tmem, k_desc + 2u * kk, q_desc + 2u * kk, idesc, kk > 0 ? 1u : 0u);
-          mma_commit(&bar->empty[s]);
+            mma_i8_ss_warp(d_tmem, k_desc + 2u * kk, q_desc + 2u * kk, idesc, kk > 0 ? 1u : 0u,
+                           elected);
+          mma_commit_warp(&bar->empty[s], elected);
         }
-        if (ok) mma_commit(&bar->tmem_full[t & 1]);
+        if (ok) mma_commit_warp(&bar->tmem_full[t & 1], elected);
       }
-      mma_commit(&bar->drain);
-      drain_wait(&bar->drain, 0);
+      mma_commit_warp(&bar->drain, elected);
+      if (lane == 0) drain_wait(&bar->drain, 0);
+      __syncwarp();
     }
   } else {
     // Warps 0-3 take the even tiles, 4-7 the odd ones: one key block per thread.
