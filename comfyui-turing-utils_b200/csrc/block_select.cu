@@ -27,7 +27,7 @@
 //      4-stage ring, warp 9 issues the MMAs into two TMEM buffers, warps 0-3
 //      and 4-7 take the tiles in turn and leave the top word of each score's
 //      sortable bits in shared memory.  Then one warp per query block finds the
-//      keep-th word (find_edge), and, where that word is shared by more blocks
+//      keep-th word (choose_row), and, where that word is shared by more blocks
 //      than fit, again with their low words from the digits.  Two CTAs per SM
 //      (up to 1300 key blocks): one's search runs under the other's products.
 #include <algorithm>
@@ -721,8 +721,9 @@ __global__ void __launch_bounds__(kSelectThreads, 2)
   int32_t* out = p.out + grow * p.keep;
   uint32_t edge = 0u;
   if (choose_row<PER_LANE>(row, blocks, p.keep, p.z, p.slope, false, out, edge)) return;
-  // Blocks share the edge's top word: their low words decide.  The digits give
-  // the same integer, so the same fp64 score, as the tensor core did.
+  // Blocks share the edge's top word: their low words decide, without the last bit
+  // (0 and ~0 are taken) and then by it.  The digits give the same integer, so the
+  // same fp64 score, as the tensor core did.
   const int8_t* qd = p.q_digits + grow * (kQDigits * kChannels) + lane * 4;
   int64_t q[4];
 #pragma unroll
@@ -732,23 +733,27 @@ __global__ void __launch_bounds__(kSelectThreads, 2)
     for (int d = kQDigits - 1; d >= 0; --d) q[c] = q[c] * 128 + qd[d * kChannels + c];
   }
   const int64_t plane = static_cast<int64_t>(p.B) * p.Hk * p.key_blocks * kChannels;
-  for (int j = 0; j < blocks; ++j) {
-    const uint32_t word = row[j];
-    uint32_t next = word > edge ? ~0u : 0u;
-    if (word == edge) {
-      const int8_t* kd = p.k_digits + (kv * p.key_blocks + j) * kChannels + lane * 4;
-      int64_t v = 0;
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    for (int j = 0; j < blocks; ++j) {
+      const uint32_t word = row[j];
+      uint32_t next = word > edge ? ~0u : 0u;
+      if (word == edge) {
+        const int8_t* kd = p.k_digits + (kv * p.key_blocks + j) * kChannels + lane * 4;
+        int64_t v = 0;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) v += q[c] * (kd[plane + c] * 128 + kd[c]);
+        for (int c = 0; c < 4; ++c) v += q[c] * (kd[plane + c] * 128 + kd[c]);
 #pragma unroll
-      for (int m = 16; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
-      next = 1u + (low_word(exact_score(v, p.k_factor[kv * p.key_blocks + j])) >> 1);
+        for (int m = 16; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+        const uint32_t low = low_word(exact_score(v, p.k_factor[kv * p.key_blocks + j]));
+        next = 1u + (pass == 0 ? low >> 1 : low & 1u);
+      }
+      __syncwarp();
+      if (lane == 0) row[j] = next;
     }
     __syncwarp();
-    if (lane == 0) row[j] = next;
+    if (choose_row<PER_LANE>(row, blocks, p.keep, p.z, p.slope, pass == 1, out, edge)) return;
   }
-  __syncwarp();
-  choose_row<PER_LANE>(row, blocks, p.keep, p.z, p.slope, true, out, edge);
 }
 
 // Quantile of the standard normal distribution by bisection of erfc: a guess's

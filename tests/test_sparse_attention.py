@@ -341,6 +341,31 @@ def test_ties_zeros_and_nan(Lk):
 
 
 @gpu
+@pytest.mark.parametrize("nkb", [2, 100, 2000])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_one_step_of_fp64_apart(nkb, sign):
+    """Channel 0 alone gives every block 127 * 2^33 * 8128, in [2^52, 2^53), where a
+    step of fp64 is one; channel 1 adds an integer below 128."""
+    q8 = torch.zeros(1, 1, 128, 128, dtype=torch.int8)
+    q8[0, 0, 0, 0] = 127 * sign
+    q8[0, 0, 16, 1] = 1
+    qs = torch.ones(1, 1, 8)
+    qs[0, 0, 1] = 2.0 ** -33
+    add = torch.randperm(max(nkb, 128), generator=torch.Generator().manual_seed(nkb))[:nkb] % 128
+    if nkb == 2:
+        add = torch.tensor([2, 3])     # equal but for the last bit
+    k8 = torch.zeros(1, 1, nkb, 64, 128, dtype=torch.int8)
+    k8[..., 0] = 127
+    k8[0, 0, :, 0, 1] = add.to(torch.int8)
+    k8 = k8.view(1, 1, nkb * 64, 128).cuda()
+    rank = sorted(range(nkb), key=lambda j: (-int(add[j]), j))
+    for keep in {1, min(37, nkb - 1), nkb // 2}:
+        got = turing_sage.select_key_blocks(q8.cuda(), qs.cuda(), k8,
+                                            torch.ones(1, 1, nkb, device="cuda"), keep)
+        assert got[0, 0, 0].tolist() == sorted(rank[:keep])
+
+
+@gpu
 @pytest.mark.parametrize("Lk", [100000, 131071, 250001])
 @pytest.mark.parametrize("keep", [1, 64, 600])
 def test_choice_over_long_contexts(Lk, keep):
