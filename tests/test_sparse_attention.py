@@ -366,6 +366,56 @@ def test_scores_one_step_of_fp64_apart(nkb, sign):
 
 
 @gpu
+@pytest.mark.parametrize("nkb", [40, 500, 2000])
+@pytest.mark.parametrize("spread", [20, 31, 34])
+def test_scores_that_cancel(nkb, spread):
+    """Key sums whose large products cancel to some 2^spread of 2^52, by integers.
+    A query channel's mean is written in base 128, a digit to a tile of tokens."""
+    g = torch.Generator().manual_seed(nkb + spread)
+    rand = lambda lo, hi, n: torch.randint(lo, hi, (n,), generator=g).tolist()
+    q = [(1 << 39) + x for x in rand(0, 1 << 37, 1)] + [0, 0] + \
+        [-(1 << 39) - x for x in rand(0, 1 << 36, 125)]
+    q[1], q[2] = (1 << spread) // 64 + 1, 1
+    sums, scores = [], []
+    for j in range(nkb):
+        S = [0] + rand(-64, 65, 1) + rand(-8000, 8000, 1) + rand(40, 64, 125)
+        S[0] = -round(sum(a * b for a, b in zip(q[3:], S[3:])) / q[0])
+        # What is left of channel 0's rounding is taken by the others' spread.
+        sums.append(S)
+        scores.append(sum(a * b for a, b in zip(q, S)))
+    q8 = torch.zeros(1, 1, 128, 128, dtype=torch.int8)
+    for c, v in enumerate(q):
+        u = v + 64 * (128 ** 6 - 1) // 127
+        for d in range(6):
+            q8[0, 0, 16 * d, c] = (u >> 7 * d) % 128 - 64
+    qs = torch.tensor([2.0 ** (7 * d) if d < 6 else 1.0 for d in range(8)]).view(1, 1, 8)
+    S = torch.tensor(sums)
+    row = torch.arange(64).view(1, 64, 1)
+    base = torch.div(S, 64, rounding_mode="floor")[:, None]
+    k8 = base + (row < (S - 64 * base[:, 0])[:, None]).long()
+    assert k8.abs().max() <= 127 and torch.equal(k8.sum(1), S)
+    k8 = k8.to(torch.int8).view(1, 1, nkb * 64, 128).cuda()
+    rank = sorted(range(nkb), key=lambda j: (-float(scores[j]), j))
+    for keep in (1, nkb // 7, nkb // 2, nkb - 1):
+        got = turing_sage.select_key_blocks(q8.cuda(), qs.cuda(), k8,
+                                            torch.ones(1, 1, nkb, device="cuda"), keep)
+        assert got[0, 0, 0].tolist() == sorted(rank[:keep])
+
+
+@gpu
+@pytest.mark.parametrize("exponents", [(-149, -126), (-130, -100), (60, 127), (-149, 127)])
+def test_scales_at_the_ends_of_fp32(exponents):
+    q8, qs = codes(1, 2, 300, 128, 16, "HND", 1)
+    k8, ks = codes(1, 2, 6400, 128, 64, "HND", 2)
+    g = torch.Generator().manual_seed(3)
+    power = torch.randint(exponents[0], exponents[1] + 1, ks.shape, generator=g).double()
+    ks = torch.exp2(power).float().cuda()
+    for keep in (1, 10, 50):
+        got = turing_sage.select_key_blocks(q8, qs, k8, ks, keep)
+        assert torch.equal(got, choose(q8, qs, k8, ks, keep, "HND"))
+
+
+@gpu
 @pytest.mark.parametrize("Lk", [100000, 131071, 250001])
 @pytest.mark.parametrize("keep", [1, 64, 600])
 def test_choice_over_long_contexts(Lk, keep):
