@@ -30,6 +30,9 @@
 //      keep-th word (choose_row), and, where that word is shared by more blocks
 //      than fit, again with their low words from the digits.  Two CTAs per SM
 //      (up to 1300 key blocks): one's search runs under the other's products.
+//      Bound by the latency of the scores' read-back and of the search, not by the
+//      tensor core: 75600 tokens x 40 heads, 1182 key blocks: 174 us, after 136 us
+//      (5.7 TB/s) of sums.
 #include <algorithm>
 #include <cmath>
 
@@ -161,7 +164,7 @@ struct ChannelSums {
 
 // Block and (batch, head) of a task, in the order that memory is laid out:
 // where a token's heads lie side by side, the heads of a block come one after
-// another.
+// another (75600 tokens x 40 heads: 136 us, 146 by heads first).
 __device__ __forceinline__ void block_of(int64_t task, int B, int H, int blocks,
                                          const int64_t (&stride)[3], int& block, int& bh) {
   if (stride[1] < stride[2]) {
@@ -793,7 +796,8 @@ void check_select(int64_t B, int64_t Hq, int64_t Hk, int64_t Lq, int64_t Lk, int
 void select_launch(SelectParams& p, cudaStream_t stream) {
   // Query blocks per CTA: fewer where their keys outgrow shared memory or where
   // the CTAs would not fill the SMs (the search is a warp per query block, the
-  // products of idle rows cost nothing that matters).
+  // products of idle rows cost nothing that matters).  8 heads, 8 query blocks, 313
+  // key blocks: 8.5 us, 9.4 with full CTAs; 12 heads, 33, 73: 7.5 and 7.2.
   const int64_t head_rows = static_cast<int64_t>(p.Hq) / p.Hk * p.query_blocks;
   const int64_t heads = static_cast<int64_t>(p.B) * p.Hk;
   auto smem_of = [&](int rows) {

@@ -19,6 +19,9 @@
 // flight.  A thread keeps one token and one pack of channels and walks over the
 // heads of Q and then K, so its sines and cosines are computed once in
 // registers and reused by every head, with no table in memory and no barrier.
+// 32760 tokens x 40 heads, interleaved: bf16 118 us (5.7 TB/s), fp32 211 us (6.4
+// TB/s).  Tensors that do not allow 16-byte packs (strides, alignment, a head or
+// rotated part that is no whole number of packs) go by single pairs: 307 and 321 us.
 #include <algorithm>
 #include <cmath>
 
@@ -259,7 +262,8 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeParams p) 
 }
 
 // out [batch, length, pairs, 2, 2] = scale * [[cos, -sin], [sin, cos]]: the
-// thread of G pairs writes 4 G values at once.
+// thread of G pairs writes 4 G values at once (16-bit types: 16 bytes; 75600 tokens x
+// 64 pairs 14.6 us, 15.6 with G = 1).
 template <typename T, int G>
 __global__ void __launch_bounds__(kRopeThreads)
     rope_freqs_kernel(const RopePositions pos, T* __restrict__ out, int length, int pairs,
@@ -357,7 +361,8 @@ void rope_launch(RopeParams& p, int64_t batch, int split_half, cudaStream_t stre
   else p.items = half + p.head_dim - p.rot_dim;
   // Threads of a CTA: items x tokens x heads.  Tokens come first (a thread's
   // sines serve all heads); heads share the CTA and then the grid where there
-  // are too few tokens to fill the SMs (4 CTAs each).
+  // are too few tokens to fill the SMs (4 CTAs each; 40 heads: 64 tokens 2.9 us, 13.4
+  // unsplit, 512 tokens 5.0 us, 7.3 with 16 CTAs each).
   p.items_cta = std::min(p.items, kRopeThreads);
   const int lanes = kRopeThreads / p.items_cta;
   p.tok_lanes = static_cast<int>(std::min<int64_t>(lanes, p.length));
@@ -389,9 +394,10 @@ void freqs_launch(const RopePositions& pos, void* out, int64_t batch, int64_t le
   const int groups = two ? pairs / 2 : pairs;
   const int groups_cta = std::min(groups, kRopeThreads);
   const int tok_lanes = kRopeThreads / groups_cta;
-  // Eight CTAs fit an SM; a few tokens per thread share its frequencies.
+  // Eight CTAs fit an SM; a thread's tokens share its frequencies (75600 tokens x 64
+  // pairs in bf16: 14.1 us, 14.6 with twice the CTAs, 21 with one token a thread).
   const int64_t blocks = (length + tok_lanes - 1) / tok_lanes;
-  const int64_t want = std::max<int64_t>(1, 16LL * device_sm_count() / batch);
+  const int64_t want = std::max<int64_t>(1, 8LL * device_sm_count() / batch);
   TB_REQUIRE(batch <= 65535, "batch exceeds the grid range");
   const dim3 grid(static_cast<unsigned>(std::min(blocks, want)),
                   static_cast<unsigned>((groups + groups_cta - 1) / groups_cta),
