@@ -113,6 +113,8 @@ def sparse_attn(query, key, value, output, query_scale, key_scale, block_index, 
         _check(output.is_cuda and output.device == device and output.shape == query.shape
                and output.dtype == value.dtype and output.stride(3) == 1,
                "output must match query's shape and value's dtype")
+        _check(all(n == 1 or s > 0 for n, s in zip(output.shape, output.stride())),
+               "output must have a place for every element")
     keep = block_index.size(3)
     size = ctypes.c_int64(0)
     _require_sm100(device)

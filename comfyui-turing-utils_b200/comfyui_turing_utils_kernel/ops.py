@@ -533,9 +533,11 @@ def turing_rope(
     The first 2 * len(inv_freq) channels of each head turn; the others are
     copied.  Pair p, channels (2p, 2p + 1) or with split_half (p, p + pairs),
     turns by position * inv_freq[p] (the angle is taken in fp64) and is
-    multiplied by scale.  positions: int32, int64, float32 or float64, [L] or
-    [1 or B, L]; with axis_pairs (pairs of each of 1 to 4 axes) [L, axes] or
-    [1 or B, L, axes].  inverse turns the other way.
+    multiplied by scale.  positions: int32, int64 (within 2^51), float32 or
+    float64, [L] or [1 or B, L]; with axis_pairs (pairs of each of 1 to 4 axes)
+    [L, axes] or [1 or B, L, axes].  inverse turns the other way.  No gradients
+    reach positions and inv_freq.  To capture a backward pass into a CUDA graph,
+    take leaves that no live eager graph holds (torch raises an error otherwise).
     """
     return _rope_call(x, None, positions, inv_freq,
                       (tensor_layout, split_half, axis_pairs, float(scale), inverse))
@@ -588,7 +590,7 @@ def turing_rope_freqs(
     dtype: torch.dtype = torch.bfloat16,
 ) -> torch.Tensor:
     """The rotations of turing_rope as matrices scale * [[cos, -sin], [sin, cos]],
-    [1 or B, L, 1, len(inv_freq), 2, 2]: the freqs argument of
+    [1 or B, L, 1, len(inv_freq), 2, 2] (B up to 65535): the freqs argument of
     turing_sage.prequantize_rms_rope_qk."""
     if _eager(positions, inv_freq):
         return _C.turing_rope_freqs(positions, inv_freq, axis_pairs, float(scale), dtype)

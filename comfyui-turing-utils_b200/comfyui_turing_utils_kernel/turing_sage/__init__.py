@@ -146,7 +146,7 @@ def sparse_sageattn_compiled(query: torch.Tensor, key: torch.Tensor, value: torc
     from .custom_ops import sparse_sage_attention
 
     return sparse_sage_attention(query, key, value, int(keep), tensor_layout,
-                                 -1.0 if sm_scale is None else float(sm_scale), bool(smooth_k),
+                                 None if sm_scale is None else float(sm_scale), bool(smooth_k),
                                  key_lengths, block_policy)
 
 

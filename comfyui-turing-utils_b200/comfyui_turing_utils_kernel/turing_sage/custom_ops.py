@@ -77,15 +77,15 @@ def _w8a8_attention_fake(query, key, value, tensor_layout, is_causal, sm_scale, 
 
 @torch.library.custom_op("turing_utils::sparse_sage_attention", mutates_args=())
 def sparse_sage_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, keep: int,
-                          tensor_layout: str, sm_scale: float, smooth_k: bool,
+                          tensor_layout: str, sm_scale: float | None, smooth_k: bool,
                           key_lengths: torch.Tensor | None,
                           block_policy: torch.Tensor | None) -> torch.Tensor:
     from .sparse import sparse_sageattn
 
     # A custom op's result is contiguous: heads below 128 come back as a slice.
     return sparse_sageattn(query, key, value, keep, tensor_layout=tensor_layout,
-                           sm_scale=sm_scale if sm_scale > 0.0 else None, smooth_k=smooth_k,
-                           key_lengths=key_lengths, block_policy=block_policy).contiguous()
+                           sm_scale=sm_scale, smooth_k=smooth_k, key_lengths=key_lengths,
+                           block_policy=block_policy).contiguous()
 
 
 @sparse_sage_attention.register_fake

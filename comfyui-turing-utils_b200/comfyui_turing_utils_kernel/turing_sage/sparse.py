@@ -41,8 +41,10 @@ def select_key_blocks(q_int8: torch.Tensor, q_scale: torch.Tensor, k_int8: torch
     min(keep, ceil(Lk / 64))], ascending, -1 where fewer blocks can be chosen.
 
     The score of a query block and a key block is the product of their mean
-    dequantized query and key, exact to fp64; the `keep` highest are taken, ties
-    to the lowest block, a NaN score last.  Positive sm_scale, K smoothing and
+    dequantized query and key; the `keep` highest are taken, ties to the lowest
+    block, a NaN score last.  The mean query is held to 2^-40 of its largest
+    channel, all else is exact up to one fp64 rounding; a query block with a scale
+    that is not finite scores 0 everywhere.  Positive sm_scale, K smoothing and
     the Hadamard rotation change no rank beyond INT8 rounding.
 
     q_int8 / k_int8 and scales: as the Sage quantizers return them (head_dim 64 or
@@ -71,7 +73,8 @@ def sparse_sageattn_prequantized(q_int8: torch.Tensor, q_scale: torch.Tensor,
     entries that name no block with visible keys are skipped, a block named twice
     counts twice.  key_lengths: int32 [B], keys from there on are not seen,
     whatever K and V hold there.  A row that sees no key is 0 (lse -inf).  lse:
-    natural logarithm, float32 [B, Hq, Lq].
+    natural logarithm, float32 [B, Hq, Lq].  output: written in place of a new
+    tensor; it must not overlap the inputs.
     """
     if q_int8.ndim != 4:
         raise ValueError("prequantized Sage Q/K/V must be four-dimensional")
@@ -94,6 +97,8 @@ def sparse_sageattn_from_prequantized(quantized: PrequantizedSageAttention, keep
     prequantize_sageattn or prequantize_sageattn_from_qk."""
     if quantized.is_causal:
         raise ValueError("causal masking is supported only by dense attention")
+    if quantized.sm_scale < 0.0:  # would turn the choice around
+        raise ValueError("sm_scale must not be negative where key blocks are chosen")
     lists = select_key_blocks(
         quantized.query_int8, quantized.query_scale, quantized.key_int8, quantized.key_scale,
         keep, tensor_layout=quantized.tensor_layout, key_lengths=key_lengths,

@@ -426,7 +426,7 @@ TB_API int tb_w8a8_attn(const int8_t *q, const int8_t *k, const void *v_codes,
  * (p, p + rot_dim / 2), turns by position * inv_freq[p] (fp64 [rot_dim / 2]),
  * by the negative angle when inverse != 0 (the gradient), and is multiplied by
  * scale.  positions: contiguous [position_batches, length, axes] of type
- * TB_POS_*, position_batches 1 (shared) or batch; axis_pairs (host, int32
+ * TB_POS_* (I64: within 2^51), position_batches 1 (shared) or batch; axis_pairs (host, int32
  * [axes], or NULL for one axis) counts the pairs that turn with each axis.
  * strides (elements, 12 values): query (b, h, l), key (b, h, l), query_out
  * (b, h, l), key_out (b, h, l); the last dimension is contiguous.  Any
@@ -443,8 +443,8 @@ TB_API int tb_rope(const void *query, const void *key, void *query_out, void *ke
 
 /* The rotations as 2x2 matrices scale * [[cos, -sin], [sin, cos]]: output
  * [batch, length, pairs, 2, 2] contiguous, 16-byte aligned, the freqs operand
- * of tb_quant_qk_rms_rope_int8 and tb_qk_rms_rope_apply.  Other arguments as
- * for tb_rope.  No counterpart in the reference. */
+ * of tb_quant_qk_rms_rope_int8 and tb_qk_rms_rope_apply; batch <= 65535.  Other
+ * arguments as for tb_rope.  No counterpart in the reference. */
 TB_API int tb_rope_freqs(const void *positions, int position_type, int64_t position_batches,
                          const double *inv_freq, const int32_t *axis_pairs, int axes,
                          void *output, int64_t batch, int64_t length, int64_t pairs, int dtype,
@@ -456,8 +456,10 @@ TB_API int tb_rope_freqs(const void *positions, int position_type, int64_t posit
  * queries attends to: block_index int32 [B, Hq, ceil(Lq/128), keep], ascending,
  * filled up with -1 where fewer blocks can be chosen.  The score of a pair is
  * the product of the mean dequantized query and the mean dequantized visible
- * key, exact to fp64; the keep highest are taken, ties to the lowest block, a
- * NaN score last.  q, k: the INT8 codes of the Sage quantizers with q_scale
+ * key (the mean query held to 2^-40 of its largest channel, all else exact up to
+ * one fp64 rounding; a query block with a scale that is not finite scores 0
+ * everywhere); the keep highest are taken, ties to the lowest block, a NaN
+ * score last.  q, k: the INT8 codes of the Sage quantizers with q_scale
  * [B, Hq, ceil(Lq/64)*4] and k_scale [B, Hk, ceil(Lk/64)]; strides (elements,
  * 6 values): q (b, h, l), k (b, h, l), multiples of 16, last dimension
  * contiguous, Q/K 16-byte aligned.  key_lengths int32 [B] or NULL: keys from
@@ -487,7 +489,7 @@ TB_API int tb_select_key_blocks(const int8_t *q, const int8_t *k, const float *q
  * key is 0.  out of V's dtype; lse: optional [B, Hq, Lq] natural log-sum-exp
  * (-inf for a row that sees no key).  strides (elements, 12 values): q, k, v,
  * out (b, h, l), Q/K multiples of 16, V/out of 8, last dimension contiguous;
- * Q/K/V/out 16-byte aligned; D = 128.  workspace: 16-byte aligned, at least the
+ * Q/K/V/out 16-byte aligned, out apart from the inputs; D = 128.  workspace: 16-byte aligned, at least the
  * bytes that tb_sparse_attn_workspace returns (0: may be NULL).  The sparse
  * counterpart of the reference's attn_cuda_sm75.h:21-31 with the caller's
  * lists in place of its Sol routes. */

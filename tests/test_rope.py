@@ -254,6 +254,54 @@ def test_streams_graphs_and_compile():
     assert torch.equal(f(new), kernel.turing_rope(new, pos, inv) * 2)
 
 
+@gpu
+def test_captured_gradients_beside_an_eager_graph():
+    """Forward and gradients captured and replayed on new values while an eager
+    graph of the same memory lives; that one still gives its own gradients.  (The
+    captured leaves are objects of their own: torch refuses to capture a backward
+    pass into leaves that a live eager graph holds, whatever the operator.)"""
+    inv, _ = kernel.turing_rope_inv_freq(64, device="cuda")
+    pos = torch.arange(65, device="cuda")
+    q = rand((1, 4, 65, 64), "HND", torch.float32, 1).requires_grad_()
+    k = rand((1, 2, 65, 64), "HND", torch.float32, 2).requires_grad_()
+    gq, gk = rand((1, 4, 65, 64), "HND", torch.float32, 3), rand((1, 2, 65, 64), "HND",
+                                                                 torch.float32, 4)
+    eager = kernel.turing_rope_qk(q, k, pos, inv)
+    want = torch.autograd.grad(eager, (q, k), (gq, gk), retain_graph=True)
+    graph = torch.cuda.CUDAGraph()
+    q2, k2 = q.detach().requires_grad_(), k.detach().requires_grad_()
+    with torch.cuda.graph(graph):
+        out = kernel.turing_rope_qk(q2, k2, pos, inv)
+        grads = torch.autograd.grad(out, (q2, k2), (gq, gk))
+    new = [rand(tuple(t.shape), "HND", torch.float32, 7 + i) for i, t in enumerate((gq, gk))]
+    old = [gq.clone(), gk.clone()]
+    gq.copy_(new[0])
+    gk.copy_(new[1])
+    graph.replay()
+    again = torch.autograd.grad(eager, (q, k), tuple(old))
+    assert torch.equal(again[0], want[0]) and torch.equal(again[1], want[1])
+    expect = torch.autograd.grad(kernel.turing_rope_qk(q, k, pos, inv), (q, k), tuple(new))
+    assert torch.equal(grads[0], expect[0]) and torch.equal(grads[1], expect[1])
+
+
+@gpu
+@pytest.mark.parametrize("split_half", [0, 1])
+def test_c_entry_in_place(split_half):
+    """An output may be its input."""
+    inv, _ = kernel.turing_rope_inv_freq(48, device="cuda")
+    pos = torch.arange(33, device="cuda")
+    for odd in (0, 1):
+        x = rand((1, 3, 33, 64), "HND", torch.bfloat16, 1)
+        room = torch.empty(x.numel() + 1, dtype=x.dtype, device="cuda")
+        y = room[odd:odd + x.numel()].view_as(x).copy_(x)
+        want = kernel.turing_rope(x, pos, inv, split_half=bool(split_half))
+        s = (ctypes.c_int64 * 12)(*((6336, 2112, 64, 0, 0, 0) * 2))
+        _lib.call("tb_rope", y.data_ptr(), None, y.data_ptr(), None, pos.data_ptr(), 1, 1,
+                  inv.data_ptr(), None, 1, 1, 3, 0, 33, 64, 48, s, split_half, 0,
+                  _lib.TB_DTYPE_BF16, 1.0, torch.cuda.current_stream().cuda_stream)
+        assert torch.equal(y, want)
+
+
 # ---------------------------------------------------------------------- CPU --
 
 def test_fake_contracts():

@@ -537,6 +537,36 @@ def test_graphs_streams_and_compile(Lq):
     assert torch.equal(f(*news[0]), want[0])
 
 
+@gpu
+@pytest.mark.parametrize("layout", ["HND", "NHD"])
+def test_keys_shared_by_expansion(layout):
+    """K and V of one batch entry and one head seen by all of them (strides of zero)
+    give what their copies give."""
+    q8, qs = codes(2, 4, 200, 128, 16, layout, 1)
+    k8, ks = codes(1, 1, 900, 128, 64, layout, 2)
+    v = value(1, 1, 900, torch.bfloat16, layout, 3)
+    ks = ks.expand(2, 4, -1)
+    shape = (2, 4, 900, 128) if layout == "HND" else (2, 900, 4, 128)
+    k8, v = k8.expand(shape), v.expand(shape)
+    lists = turing_sage.select_key_blocks(q8, qs, k8, ks, 5, tensor_layout=layout)
+    assert torch.equal(lists, turing_sage.select_key_blocks(q8, qs, k8.contiguous(), ks, 5,
+                                                            tensor_layout=layout))
+    got, want = (turing_sage.sparse_sageattn_prequantized(q8, qs, a, ks, b, lists,
+                                                          tensor_layout=layout)
+                 for a, b in ((k8, v), (k8.contiguous(), v.contiguous())))
+    assert torch.equal(got, want)
+
+
+@gpu
+def test_compiled_leaf_keeps_every_scale():
+    q, k, v = (value(1, 2, n, torch.bfloat16, "HND", s) for n, s in ((130, 1), (700, 2), (700, 3)))
+    for scale in (None, 0.0, 0.3):
+        assert torch.equal(turing_sage.sparse_sageattn_compiled(q, k, v, 4, sm_scale=scale),
+                           turing_sage.sparse_sageattn(q, k, v, 4, sm_scale=scale))
+    with pytest.raises(ValueError, match="negative"):
+        turing_sage.sparse_sageattn_compiled(q, k, v, 4, sm_scale=-0.3)
+
+
 # --------------------------------------------------------------------- CPU --
 
 class FakeCuda(torch.Tensor):
@@ -614,6 +644,15 @@ def test_other_refusals():
                                        "HND", 128, True, 1.0)
     with pytest.raises(ValueError, match="causal"):
         turing_sage.sparse_sageattn_from_prequantized(causal, 1)
+    turned = PrequantizedSageAttention(cpu, torch.ones((1, 1, 4)), cpu, torch.ones((1, 1, 1)), x,
+                                       "HND", 128, False, -1.0)
+    with pytest.raises(ValueError, match="negative"):
+        turing_sage.sparse_sageattn_from_prequantized(turned, 1)
+    with pytest.raises(RuntimeError, match="a place for every element"):
+        turing_sage.sparse_sageattn_prequantized(
+            **good(), v=fake(2, 2, 200, 128, dtype=torch.float16),
+            block_index=fake(2, 4, 2, 3, dtype=torch.int32),
+            output=fake(1, 4, 130, 128, dtype=torch.float16).expand(2, 4, 130, 128))
 
 
 def test_fake_contract():
