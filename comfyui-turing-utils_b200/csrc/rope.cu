@@ -396,7 +396,8 @@ void freqs_launch(const RopePositions& pos, void* out, int64_t batch, int64_t le
   const int tok_lanes = kRopeThreads / groups_cta;
   // Eight CTAs fit an SM; two rounds of them, whose tokens share a thread's
   // frequencies (75600 tokens x 64 pairs in bf16, a call on memory not in L2: 16.5 us,
-  // 18.2 with one round, 18.4 with four; one token a thread 44 % longer than this).
+  // 18.2 with one round, 18.4 with four; in a loop over memory in L2 one token a
+  // thread takes 44 % longer than two rounds).
   const int64_t blocks = (length + tok_lanes - 1) / tok_lanes;
   const int64_t want = std::max<int64_t>(1, 16LL * device_sm_count() / batch);
   TB_REQUIRE(batch <= 65535, "batch exceeds the grid range");

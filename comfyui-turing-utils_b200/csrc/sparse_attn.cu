@@ -34,7 +34,10 @@
 // So what can overlap them does: the second half of S loads under the first
 // half's exponentials and the first half of the next block's S while P is stored,
 // the producer follows the list and fetches the K scales, the issuer has looked
-// at the rings before P comes, and everything rare is out of the way.
+// at the rings before P comes, and everything rare is out of the way.  Taking an
+// eighth or a quarter of the exponentials off their unit by a polynomial costs more
+// issue slots than it frees (32760 tokens x 40 heads, 64 blocks a list: 2.17 ms,
+// 2.25 and 2.35 with it; medians of three).
 //
 // Few query blocks (single tokens): the list is split over CTAs, which write
 // unnormalized O, m and d; sparse_combine_kernel joins them.
