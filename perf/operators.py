@@ -21,18 +21,13 @@ QB, KB, D = 128, 64, 128        # query block, key block, channels of a head
 DTYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
 
 
-_kernel = None
-
-
 def _package():
-    """The package, imported once as a user's program does."""
-    global _kernel
-    if _kernel is None:
-        pkg = str(Path(__file__).resolve().parents[1] / "comfyui-turing-utils_b200")
-        if pkg not in sys.path:
-            sys.path.insert(1, pkg)
-        import comfyui_turing_utils_kernel as _kernel
-    return _kernel
+    pkg = str(Path(__file__).resolve().parents[1] / "comfyui-turing-utils_b200")
+    if pkg not in sys.path:
+        sys.path.insert(1, pkg)
+    import comfyui_turing_utils_kernel as kernel
+
+    return kernel
 
 
 # ------------------------------------------------------------------- cases --
