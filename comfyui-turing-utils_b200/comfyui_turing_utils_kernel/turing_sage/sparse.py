@@ -74,7 +74,8 @@ def sparse_sageattn_prequantized(q_int8: torch.Tensor, q_scale: torch.Tensor,
     counts twice.  key_lengths: int32 [B], keys from there on are not seen,
     whatever K and V hold there.  A row that sees no key is 0 (lse -inf).  lse:
     natural logarithm, float32 [B, Hq, Lq].  output: written in place of a new
-    tensor; it must not overlap the inputs.
+    tensor; it must not overlap the inputs.  sm_scale and the scales may have
+    either sign.
     """
     if q_int8.ndim != 4:
         raise ValueError("prequantized Sage Q/K/V must be four-dimensional")

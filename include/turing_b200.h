@@ -486,8 +486,9 @@ TB_API int tb_select_key_blocks(const int8_t *q, const int8_t *k, const float *q
  * (negative, too large, at or past key_lengths) are skipped, a block named
  * twice counts twice.  Keys from key_lengths[b] (int32 [B] or NULL, clamped to
  * 0 .. Lk) on are not seen, whatever K and V hold there.  A row that sees no
- * key is 0.  out of V's dtype; lse: optional [B, Hq, Lq] natural log-sum-exp
- * (-inf for a row that sees no key).  strides (elements, 12 values): q, k, v,
+ * key is 0.  sm_scale and the scales may have either sign.  out of V's dtype;
+ * lse: optional [B, Hq, Lq] natural log-sum-exp (-inf for a row that sees no key).
+ * strides (elements, 12 values): q, k, v,
  * out (b, h, l), Q/K multiples of 16, V/out of 8, last dimension contiguous;
  * Q/K/V/out 16-byte aligned, out apart from the inputs; D = 128.  workspace: 16-byte aligned, at least the
  * bytes that tb_sparse_attn_workspace returns (0: may be NULL).  The sparse

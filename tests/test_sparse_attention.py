@@ -188,6 +188,38 @@ def test_scales(spread, gain, Lq):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Lq", [1, 200])
+@pytest.mark.parametrize("where", ["sm_scale", "query", "key", "both"])
+def test_negative_scales(dtype, Lq, where):
+    """A negative sm_scale, negative scales of some query tiles (two tiles share a
+    warp) or key blocks: the row's largest score is then the smallest integer one.
+    Logits of either sign up to tens, as in test_scales."""
+    q8, qs = codes(1, 4, Lq, 128, 16, "HND", 1, math.sqrt(30.0))
+    k8, ks = codes(1, 2, 1500, 128, 64, "HND", 2, math.sqrt(30.0))
+    v = value(1, 2, 1500, dtype, "HND", 3)
+    lists = random_lists(1, 4, Lq, 1500, 20, 4)
+    sm_scale = 128 ** -0.5
+    if where == "sm_scale":
+        sm_scale = -sm_scale
+    if where in ("query", "both"):
+        qs[..., ::2] *= -1
+    if where in ("key", "both"):
+        ks[..., 1::3] *= -1
+    out, lse = turing_sage.sparse_sageattn_prequantized(q8, qs, k8, ks, v, lists,
+                                                        sm_scale=sm_scale, return_lse=True)
+    o, A, want = reference(q8, qs, k8, ks, v, lists, "HND", sm_scale=sm_scale)
+    top = (dequant(q8, qs, 16, "HND") @ dequant(k8, ks, 64, "HND").repeat_interleave(
+        2, dim=1).transpose(2, 3)).abs().max().item() * 128 ** -0.5
+    grow = 2 * 4 * top * 2.0 ** -24
+    bound = (HALF_STEP[dtype] + 5.3e-4 + grow) * A + HALF_STEP[dtype] * o.abs() + (
+        20 * 64 * 2.0 ** -25 * 6.0 if dtype == torch.float16 else 0.0)
+    err = (out.double() - o).abs()
+    assert (err <= bound).all(), (err - bound).max().item()
+    assert ((lse.double() - want).abs() <= 5.3e-4 + grow + 2.0 ** -22 * want.abs()).all()
+
+
+@gpu
 def test_small_scores_in_blocks_of_large_scale():
     """Queries whose codes are small beside their tile's largest: the scores are
     small integers times a large factor, exact for every key."""
