@@ -835,8 +835,10 @@ void select_launch(SelectParams& p, cudaStream_t stream) {
   }
   const size_t smem = smem_of(p.rows_cta);
   auto launch = [&](auto kern) {
+    // The limit is the kernel's, shared by all host threads: always the same value, or
+    // one thread's shorter row would refuse another's launch.
     TB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(smem)));
+                                       static_cast<int>(device_smem_optin())));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(heads * p.groups * p.cluster));
     cfg.blockDim = dim3(kSelectThreads);

@@ -471,6 +471,44 @@ def test_choice_reads_views():
     assert torch.equal(a, b)
 
 
+@gpu
+def test_choice_from_two_threads():
+    """Host threads, each on a stream of its own, choose blocks of different lengths:
+    another shared memory size of the same kernel."""
+    import threading
+
+    lib, cases, errors = _lib.load(), [], []
+    for Lk in (6400, 16000, 4160, 17000):
+        q8, qs = codes(1, 2, 200, 128, 16, "HND", 1)
+        k8, ks = codes(1, 2, Lk, 128, 64, "HND", 2)
+        want = turing_sage.select_key_blocks(q8, qs, k8, ks, 7)
+        size = ctypes.c_int64(0)
+        assert lib.tb_select_key_blocks_workspace(1, 2, 2, 200, Lk, 128, ctypes.byref(size)) == 0
+        room = torch.empty(size.value, dtype=torch.uint8, device="cuda")
+        strides = (ctypes.c_int64 * 6)(0, 200 * 128, 128, 0, Lk * 128, 128)
+        cases.append((Lk, q8, qs, k8, ks, want, torch.zeros_like(want), room, strides,
+                      torch.cuda.Stream()))
+    torch.cuda.synchronize()
+
+    def work(Lk, q8, qs, k8, ks, want, got, room, strides, stream):
+        for _ in range(4000):
+            if lib.tb_select_key_blocks(
+                    q8.data_ptr(), k8.data_ptr(), qs.data_ptr(), ks.data_ptr(), None, None, 0,
+                    got.data_ptr(), room.data_ptr(), room.numel(), 1, 2, 2, 200, Lk, 128, 7,
+                    strides, stream.cuda_stream) != 0:
+                errors.append(_lib.last_error())
+                return
+
+    threads = [threading.Thread(target=work, args=c) for c in cases]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    assert all(torch.equal(c[6], c[5]) for c in cases)
+
+
 # ---------------------------------------------------------------- together --
 
 @gpu
