@@ -349,8 +349,8 @@ def turing_rope_inv_freq(
       "ntk"     raises theta to theta * factor^(n / (n - 1)), which keeps the
                 fastest frequency and divides the slowest by factor;
       "yarn"    divides the frequencies that turn less than beta_slow times in
-                original_length tokens, keeps those above beta_fast turns, blends
-                linearly in the pair index between, and scales by
+                original_length tokens, keeps those above beta_fast turns (and always
+                the first), blends linearly in the pair index between, and scales by
                 0.1 ln(factor) + 1.
     Otherwise the scale is 1.
     """
@@ -378,7 +378,8 @@ def turing_rope_inv_freq(
             def pair_of(turns):  # the pair that turns this often in original_length
                 return n * math.log(original_length / (turns * 2.0 * math.pi)) / math.log(theta)
             low = max(math.floor(pair_of(beta_fast)), 0)
-            high = min(math.ceil(pair_of(beta_slow)), n - 1)
+            # Pairs are counted in 2 n channels: the ramp may end past the last one.
+            high = min(math.ceil(pair_of(beta_slow)), 2 * n - 1)
             slow = ((i - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
             f = f * (1.0 - slow) + f / factor * slow
         freqs.append(f)

@@ -8,6 +8,7 @@ each (3 x 0.6e-7): 4e-7 s (|x0| + |x1|); then half a step of the output type.
 from __future__ import annotations
 
 import ctypes
+import math
 
 import pytest
 import torch
@@ -335,6 +336,37 @@ def test_inv_freq():
     axes, _ = kernel.turing_rope_inv_freq(16, axis_pairs=[4, 0, 1, 3])
     torch.testing.assert_close(axes[:4], inv)
     assert axes[4] == 1.0
+
+
+@pytest.mark.parametrize("rot,theta,length,factor,beta_fast,beta_slow,axis_pairs", [
+    (128, 10000.0, 4096, 8.0, 32.0, 1.0, None), (128, 10000.0, 65536, 4.0, 32.0, 1.0, None),
+    (128, 10000.0, 131072, 8.0, 32.0, 1.0, None), (16, 10000.0, 32768, 4.0, 32.0, 1.0, None),
+    (64, 500000.0, 8192, 2.5, 16.0, 0.5, None), (128, 10000.0, 65536, 4.0, 32.0, 1.0, [22, 21, 21]),
+    (2, 10000.0, 4096, 4.0, 32.0, 1.0, None), (128, 100.0, 1 << 24, 4.0, 32.0, 1.0, None)])
+def test_yarn_frequencies(rot, theta, length, factor, beta_fast, beta_slow, axis_pairs):
+    """The published ramp, pair by pair: its ends are the pairs (of d = 2 n channels)
+    that turn beta_fast and beta_slow times, rounded outwards and kept in 0 .. d - 1.
+    Where both lie inside, a pair that turns more than beta_slow times is never
+    divided by the whole factor."""
+    inv, scale = kernel.turing_rope_inv_freq(rot, theta, axis_pairs=axis_pairs, scaling="yarn",
+                                             factor=factor, original_length=length,
+                                             beta_fast=beta_fast, beta_slow=beta_slow)
+    want = []
+    for n in axis_pairs or [rot // 2]:
+        d = 2 * n
+
+        def pair(turns):
+            return d * math.log(length / (turns * 2 * math.pi)) / (2 * math.log(theta))
+
+        low, high = max(math.floor(pair(beta_fast)), 0), min(math.ceil(pair(beta_slow)), d - 1)
+        for i in range(n):
+            f = theta ** (-2 * i / d)
+            ramp = min(max((i - low) / (high - low if high > low else 1e-3), 0.0), 1.0)
+            want.append(f / factor * ramp + f * (1 - ramp))
+            if f * length / (2 * math.pi) > beta_slow * 1.001:
+                assert want[-1] > f / factor
+    torch.testing.assert_close(inv, torch.tensor(want, dtype=torch.float64), rtol=1e-12, atol=0)
+    assert scale == 0.1 * math.log(factor) + 1.0
 
 
 @pytest.mark.parametrize("kw,match", [
