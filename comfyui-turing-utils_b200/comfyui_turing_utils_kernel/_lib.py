@@ -92,6 +92,8 @@ SIGNATURES: dict[str, list] = {
     "tb_sparse_attn_workspace": [_i64, _i64, _i64, _i64, _p],
     "tb_sparse_attn": [_p, _p, _p, _int, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64,
                        _i64, _i64, _i64, _p, ctypes.c_float, _p],
+    "tb_smoothed_lse": [_p, _p, _p, _int, _p, _i64, _i64, _i64, _i64, _i64, _p, ctypes.c_float,
+                        _p],
 }
 
 _lock = threading.Lock()

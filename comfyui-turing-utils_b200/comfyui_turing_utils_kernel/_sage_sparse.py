@@ -93,9 +93,9 @@ def select_key_blocks(query, key, query_scale, key_scale, key_lengths, block_pol
 
 
 def sparse_attn(query, key, value, output, query_scale, key_scale, block_index, key_lengths,
-                layout, sm_scale, return_lse):
+                layout, sm_scale, return_lse, key_mean=None):
     """Writes the attention into output (or a new tensor); returns (output, natural
-    log-sum-exp or None)."""
+    log-sum-exp or None), with the scores of key_mean added to the latter."""
     device, B, Hq, Hk, Lq, Lk, D = _geometry(query, key, query_scale, key_scale, layout)
     _check(D == 128, "the sparse attention kernel takes head_dim 128 (pad smaller heads)")
     _check(value.is_cuda and value.device == device and value.shape == key.shape
@@ -115,6 +115,11 @@ def sparse_attn(query, key, value, output, query_scale, key_scale, block_index, 
                "output must match query's shape and value's dtype")
         _check(all(n == 1 or s > 0 for n, s in zip(output.shape, output.stride())),
                "output must have a place for every element")
+    if key_mean is not None:
+        _check(key_mean.is_cuda and key_mean.device == device and key_mean.shape == (B, Hk, D)
+               and key_mean.dtype in (torch.float16, torch.bfloat16) and key_mean.is_contiguous(),
+               "key_mean must be a contiguous float16 or bfloat16 [B, Hk, D] tensor on the "
+               "query's device")
     keep = block_index.size(3)
     size = ctypes.c_int64(0)
     _require_sm100(device)
@@ -135,4 +140,8 @@ def sparse_attn(query, key, value, output, query_scale, key_scale, block_index, 
              block_index.data_ptr(), lengths, None if lse is None else lse.data_ptr(),
              None if workspace is None else workspace.data_ptr(), size.value, B, Hq, Hk, Lq, Lk,
              D, keep, strides, float(sm_scale), raw_stream(device))
+        if lse is not None and key_mean is not None:
+            call("tb_smoothed_lse", query.data_ptr(), query_scale.data_ptr(), key_mean.data_ptr(),
+                 dtype_code(key_mean), lse.data_ptr(), B, Hq, Hk, Lq, D, strides, float(sm_scale),
+                 raw_stream(device))
     return output, lse

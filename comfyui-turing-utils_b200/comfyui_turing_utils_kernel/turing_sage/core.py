@@ -27,7 +27,7 @@ from typing import Any, Optional
 import torch
 
 from .. import _sage_qattn_sm75 as _qattn
-from .quant import per_warp_int8, per_warp_int8_hadamard
+from .quant import key_token_mean, per_warp_int8, per_warp_int8_hadamard
 
 
 @dataclass(frozen=True, slots=True)
@@ -41,6 +41,8 @@ class PrequantizedSageAttention:
     original_head_dim: int
     is_causal: bool
     sm_scale: float
+    key_mean: Optional[torch.Tensor] = None  # [B, Hk, 128] that smooth_k took off K
+    key_anchored: bool = False  # stabilize_k may have taken an anchor row off K
 
 
 @dataclass(frozen=True, slots=True)
@@ -53,6 +55,7 @@ class PrequantizedQK:
     input_dtype: torch.dtype
     original_head_dim: int
     route_original_basis: bool = False
+    key_anchored: bool = False
 
 
 def _on_input_device(function):
@@ -110,10 +113,11 @@ def prequantize_sageattn(q, k, v, tensor_layout: str = "HND", is_causal: bool = 
     if q.stride(-1) != 1 or k.stride(-1) != 1 or v.stride(-1) != 1:
         raise ValueError("the last Q/K/V dimension must be contiguous")
     scale = float(sm_scale) if sm_scale is not None else head_dim ** -0.5
+    key_mean = key_token_mean(k, tensor_layout) if smooth_k else None
     q_int8, q_scale, k_int8, k_scale = per_warp_int8(q, k, tensor_layout=tensor_layout,
-                                                     smooth_k=smooth_k)
+                                                     smooth_k=smooth_k, key_mean=key_mean)
     return PrequantizedSageAttention(q_int8, q_scale, k_int8, k_scale, v.contiguous(),
-                                     tensor_layout, head_dim, bool(is_causal), scale)
+                                     tensor_layout, head_dim, bool(is_causal), scale, key_mean)
 
 
 @_on_input_device
@@ -164,7 +168,8 @@ def sageattn(q, k, v, tensor_layout: str = "HND", is_causal: bool = False,
              sm_scale: Optional[float] = None, return_lse: bool = False, smooth_k: bool = False,
              **kwargs: Any):
     """Sage INT8 attention: per-warp INT8 Q, per-block INT8 K (optionally mean
-    smoothed), 16-bit PV with fp32 accumulation (core.py:543-570)."""
+    smoothed), 16-bit PV with fp32 accumulation (core.py:543-570).  With smooth_k
+    the lse is that of the scores against K minus its token mean."""
     quantized = prequantize_sageattn.__wrapped__(q, k, v, tensor_layout=tensor_layout,
                                                  is_causal=is_causal, sm_scale=sm_scale,
                                                  smooth_k=smooth_k)
@@ -206,7 +211,7 @@ def prequantize_rms_rope_qk(q, k, q_norm, k_norm, freqs, *, epsilon: float, rot_
         tensor_layout=tensor_layout, norm_scope=norm_scope, split_half=bool(split_half),
         rotate_qk=bool(rotate_qk), stabilize_k=bool(stabilize_k))
     return PrequantizedQK(q_int8, q_scale, k_int8, k_scale, tensor_layout, q.dtype, head_dim,
-                          bool(rotate_qk))
+                          bool(rotate_qk), bool(rotate_qk and stabilize_k))
 
 
 def prequantize_sageattn_from_qk(qk: PrequantizedQK, value: torch.Tensor, *,
@@ -238,7 +243,8 @@ def prequantize_sageattn_from_qk(qk: PrequantizedQK, value: torch.Tensor, *,
         value = torch.nn.functional.pad(value, (0, padding))
     return PrequantizedSageAttention(q_int8, qk.query_scale, k_int8, qk.key_scale,
                                      value.contiguous(), qk.tensor_layout,
-                                     qk.original_head_dim, bool(is_causal), scale)
+                                     qk.original_head_dim, bool(is_causal), scale,
+                                     key_anchored=qk.key_anchored)
 
 
 

@@ -28,20 +28,28 @@ def quantize_query_per_warp(q: torch.Tensor, BLKQ: int = 64, WARPQ: int = 16,
     return q_int8, q_scale
 
 
+def key_token_mean(k: torch.Tensor, tensor_layout: str = "HND") -> torch.Tensor:
+    """The per-channel token mean [B, H, D] that K smoothing takes off."""
+    batch, heads, _ = _geometry(k, tensor_layout)
+    mean = torch.empty((batch, heads, k.size(-1)), dtype=k.dtype, device=k.device)
+    _fused.token_mean_cuda(k, mean, 0 if tensor_layout == "NHD" else 1)
+    return mean
+
+
 def quantize_key_per_block(k: torch.Tensor, BLKK: int = 64, tensor_layout: str = "HND",
-                           smooth_k: bool = False):
+                           smooth_k: bool = False, key_mean: torch.Tensor | None = None):
     """Per-block INT8 K.  smooth_k=True subtracts the per-channel token mean
-    first (softmax-invariant K smoothing); the reference ships this arithmetic
-    (fused.cu:97-128) but leaves it unwired."""
+    (key_mean, computed here where None) first (softmax-invariant K smoothing); the
+    reference ships this arithmetic (fused.cu:97-128) but leaves it unwired."""
     k_int8 = torch.empty(k.shape, dtype=torch.int8, device=k.device)
     batch, heads, tokens = _geometry(k, tensor_layout)
     k_scale = torch.empty((batch, heads, (tokens + BLKK - 1) // BLKK), device=k.device,
                           dtype=torch.float32)
     layout_id = 0 if tensor_layout == "NHD" else 1
     if smooth_k:
-        mean = torch.empty((batch, heads, k.size(-1)), dtype=k.dtype, device=k.device)
-        _fused.token_mean_cuda(k, mean, layout_id)
-        _fused.quant_per_block_int8_smooth_cuda(k, k_int8, k_scale, mean, BLKK, layout_id)
+        if key_mean is None:
+            key_mean = key_token_mean(k, tensor_layout)
+        _fused.quant_per_block_int8_smooth_cuda(k, k_int8, k_scale, key_mean, BLKK, layout_id)
     else:
         _fused.quant_per_block_int8_cuda(k, k_int8, k_scale, BLKK, layout_id)
     return k_int8, k_scale
@@ -49,10 +57,11 @@ def quantize_key_per_block(k: torch.Tensor, BLKK: int = 64, tensor_layout: str =
 
 def per_warp_int8(q: torch.Tensor, k: torch.Tensor, BLKQ: int = 64, WARPQ: int = 16,
                   BLKK: int = 64, tensor_layout: str = "HND", fuse_qk: bool = False,
-                  smooth_k: bool = False):
+                  smooth_k: bool = False, key_mean: torch.Tensor | None = None):
     """Quantize Q per warp and K per block (quant.py:140-179)."""
     q_int8, q_scale = quantize_query_per_warp(q, BLKQ, WARPQ, tensor_layout)
-    k_int8, k_scale = quantize_key_per_block(k, BLKK, tensor_layout, smooth_k=smooth_k)
+    k_int8, k_scale = quantize_key_per_block(k, BLKK, tensor_layout, smooth_k=smooth_k,
+                                             key_mean=key_mean)
     return q_int8, q_scale, k_int8, k_scale
 
 

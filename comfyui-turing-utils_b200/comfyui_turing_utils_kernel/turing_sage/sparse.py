@@ -65,7 +65,8 @@ def sparse_sageattn_prequantized(q_int8: torch.Tensor, q_scale: torch.Tensor,
                                  sm_scale: Optional[float] = None,
                                  key_lengths: Optional[torch.Tensor] = None,
                                  return_lse: bool = False,
-                                 output: Optional[torch.Tensor] = None):
+                                 output: Optional[torch.Tensor] = None,
+                                 key_mean: Optional[torch.Tensor] = None):
     """Softmax attention of each query block over the key blocks its list names.
 
     q_int8, k_int8: head_dim 128 (pad smaller heads); v: float16 or bfloat16 of
@@ -73,7 +74,9 @@ def sparse_sageattn_prequantized(q_int8: torch.Tensor, q_scale: torch.Tensor,
     entries that name no block with visible keys are skipped, a block named twice
     counts twice.  key_lengths: int32 [B], keys from there on are not seen,
     whatever K and V hold there.  A row that sees no key is 0 (lse -inf).  lse:
-    natural logarithm, float32 [B, Hq, Lq].  output: written in place of a new
+    natural logarithm, float32 [B, Hq, Lq], of the scores of the codes; for codes of
+    a smoothed K give key_mean, the [B, Hk, 128] mean taken off, and it is that of the
+    scores against K itself.  output: written in place of a new
     tensor; it must not overlap the inputs.  sm_scale and the scales may have
     either sign.
     """
@@ -86,7 +89,7 @@ def sparse_sageattn_prequantized(q_int8: torch.Tensor, q_scale: torch.Tensor,
         _unit_rows(q_int8), _unit_rows(k_int8), _unit_rows(v), output, q_scale.contiguous(),
         k_scale.contiguous(), block_index.contiguous(),
         None if key_lengths is None else key_lengths.contiguous(), _layout_id(tensor_layout),
-        scale, return_lse)
+        scale, return_lse, None if key_mean is None else key_mean.contiguous())
     return (output, lse) if return_lse else output
 
 
@@ -95,11 +98,15 @@ def sparse_sageattn_from_prequantized(quantized: PrequantizedSageAttention, keep
                                       block_policy: Optional[torch.Tensor] = None,
                                       return_lse: bool = False):
     """select_key_blocks, then the attention over its lists, for the codes of
-    prequantize_sageattn or prequantize_sageattn_from_qk."""
+    prequantize_sageattn or prequantize_sageattn_from_qk.  The lse counts the mean
+    that smoothing took off K; for codes made with stabilize_k, whose anchor is not
+    kept, it is refused."""
     if quantized.is_causal:
         raise ValueError("causal masking is supported only by dense attention")
     if quantized.sm_scale < 0.0:  # would turn the choice around
         raise ValueError("sm_scale must not be negative where key blocks are chosen")
+    if return_lse and quantized.key_anchored:
+        raise ValueError("return_lse needs codes made without stabilize_k")
     lists = select_key_blocks(
         quantized.query_int8, quantized.query_scale, quantized.key_int8, quantized.key_scale,
         keep, tensor_layout=quantized.tensor_layout, key_lengths=key_lengths,
@@ -107,7 +114,8 @@ def sparse_sageattn_from_prequantized(quantized: PrequantizedSageAttention, keep
     result = sparse_sageattn_prequantized(
         quantized.query_int8, quantized.query_scale, quantized.key_int8, quantized.key_scale,
         quantized.value, lists, tensor_layout=quantized.tensor_layout,
-        sm_scale=quantized.sm_scale, key_lengths=key_lengths, return_lse=return_lse)
+        sm_scale=quantized.sm_scale, key_lengths=key_lengths, return_lse=return_lse,
+        key_mean=quantized.key_mean)
     output, lse = result if return_lse else (result, None)
     output = output[..., :quantized.original_head_dim]
     return (output, lse) if return_lse else output

@@ -639,6 +639,60 @@ __global__ void __launch_bounds__(kCombineWarps * 32) sparse_combine_kernel(cons
     p.lse[flat] = d == 0.0f ? -INFINITY : (M + log2f(d)) * 0.6931471805599453f;
 }
 
+// lse += sm_scale * q_scale * (Q8 . mean) of each row: the part of every score that
+// K smoothing took off (the scores of the codes are those against K - mean).  Eight
+// lanes a row, 16 channels each; the products are exact in fp32.  Bound by the bytes
+// of Q8 and the lse.
+constexpr int kShiftThreads = 256;
+constexpr int kShiftLanes = kDim / 16;
+
+template <typename TM>
+__global__ void __launch_bounds__(kShiftThreads)
+    smoothed_lse_kernel(const int8_t* q, int64_t q_sb, int64_t q_sh, int64_t q_sl,
+                        const float* q_scale, const TM* mean, float* lse, int64_t rows, int Hq,
+                        int Lq, int groups, int q_tiles_scale, float sm_scale) {
+  const int64_t flat =
+      static_cast<int64_t>(blockIdx.x) * (kShiftThreads / kShiftLanes) + threadIdx.x / kShiftLanes;
+  const int part = threadIdx.x % kShiftLanes;
+  float sum = 0.0f;
+  int bh = 0, row = 0;
+  if (flat < rows) {
+    bh = static_cast<int>(flat / Lq);
+    row = static_cast<int>(flat - static_cast<int64_t>(bh) * Lq);
+    const int b = bh / Hq, h = bh % Hq;
+    const uint4 x = *reinterpret_cast<const uint4*>(q + b * q_sb + h * q_sh + row * q_sl +
+                                                    part * 16);
+    const uint4* m = reinterpret_cast<const uint4*>(
+        mean + static_cast<int64_t>(b * (Hq / groups) + h / groups) * kDim + part * 16);
+    const uint4 m0 = __ldg(m), m1 = __ldg(m + 1);
+    const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
+    const uint32_t mw[8] = {m0.x, m0.y, m0.z, m0.w, m1.x, m1.y, m1.z, m1.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float lo, hi;
+      if constexpr (std::is_same<TM, __nv_bfloat16>::value) {
+        lo = __uint_as_float(mw[i] << 16);
+        hi = __uint_as_float(mw[i] & 0xffff0000u);
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&mw[i]));
+        lo = f.x;
+        hi = f.y;
+      }
+      const uint32_t two = xw[i / 2] >> (16 * (i & 1));
+      sum = fmaf(static_cast<float>(static_cast<int8_t>(two)), lo, sum);
+      sum = fmaf(static_cast<float>(static_cast<int8_t>(two >> 8)), hi, sum);
+    }
+  }
+#pragma unroll
+  for (int i = kShiftLanes / 2; i > 0; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
+  if (flat < rows && part == 0) {
+    const float scale =
+        sm_scale * __ldg(q_scale + static_cast<int64_t>(bh) * q_tiles_scale + row / 16);
+    // A row that saw no key stays -inf.
+    if (lse[flat] != -INFINITY) lse[flat] = fmaf(scale, sum, lse[flat]);
+  }
+}
+
 // CTAs that share one list: as many as fill two per SM, each with at least
 // four blocks (one full ring).  With the join, one token of 32 heads, 64 blocks:
 // 22.5 us, whole 52.4; 300 tokens of 8 heads, 16 blocks: 18.0 us, whole 19.7, at
@@ -766,5 +820,44 @@ extern "C" int tb_sparse_attn(const int8_t* q, const int8_t* k, const void* v, i
       launch(sparse_attn_kernel<__nv_bfloat16>, sparse_combine_kernel<__nv_bfloat16>);
     else
       launch(sparse_attn_kernel<__half>, sparse_combine_kernel<__half>);
+  });
+}
+
+extern "C" int tb_smoothed_lse(const int8_t* q, const float* q_scale, const void* key_mean,
+                               int mean_dtype, float* lse, int64_t B, int64_t Hq, int64_t Hk,
+                               int64_t Lq, int64_t D, const int64_t* strides, float sm_scale,
+                               tb_stream_t stream) {
+  return guarded([&] {
+    using namespace tb;
+    TB_REQUIRE(q && q_scale && key_mean && lse && strides,
+               "query, its scales, key_mean and lse must be CUDA tensors");
+    TB_REQUIRE(D == kDim, "the smoothed log-sum-exp takes head_dim 128 (pad smaller heads)");
+    TB_REQUIRE(mean_dtype == TB_DTYPE_BF16 || mean_dtype == TB_DTYPE_F16,
+               "key_mean must be float16 or bfloat16");
+    check_geometry(B, Hq, Lq, 1);
+    TB_REQUIRE(Hk > 0 && Hq % Hk == 0, "num_qo_heads must be divisible by num_kv_heads");
+    TB_REQUIRE(std::isfinite(sm_scale), "sm_scale must be finite");
+    auto aligned = [](const void* ptr, uintptr_t a) {
+      return (reinterpret_cast<uintptr_t>(ptr) & (a - 1)) == 0;
+    };
+    TB_REQUIRE(aligned(q, 16) && aligned(key_mean, 16), "Q and key_mean must be 16-byte aligned");
+    TB_REQUIRE(aligned(q_scale, 4) && aligned(lse, 4), "scales and lse must be 4-byte aligned");
+    for (int i = 0; i < 3; ++i)
+      TB_REQUIRE(strides[i] % 16 == 0, "Q strides must be multiples of 16 bytes");
+    require_sm100();
+    const int64_t rows = B * Hq * Lq;
+    constexpr int kRowsCta = kShiftThreads / kShiftLanes;
+    const int64_t ctas = (rows + kRowsCta - 1) / kRowsCta;
+    TB_REQUIRE(ctas <= INT32_MAX, "batch, heads and queries exceed the grid range");
+    auto launch = [&](auto kern, auto* mean) {
+      kern<<<static_cast<unsigned>(ctas), kShiftThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+          q, strides[0], strides[1], strides[2], q_scale, mean, lse, rows, static_cast<int>(Hq),
+          static_cast<int>(Lq), static_cast<int>(Hq / Hk), static_cast<int>((Lq + 63) / 64 * 4),
+          sm_scale);
+      TB_CUDA_CHECK(cudaGetLastError());
+    };
+    if (mean_dtype == TB_DTYPE_BF16)
+      launch(smoothed_lse_kernel<__nv_bfloat16>, static_cast<const __nv_bfloat16*>(key_mean));
+    else launch(smoothed_lse_kernel<__half>, static_cast<const __half*>(key_mean));
   });
 }

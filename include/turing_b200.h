@@ -503,6 +503,16 @@ TB_API int tb_sparse_attn(const int8_t *q, const int8_t *k, const void *v, int v
                           int64_t Lk, int64_t D, int64_t keep, const int64_t *strides,
                           float sm_scale, tb_stream_t stream);
 
+/* Adds sm_scale * (dequantized query . key_mean) to the lse of each row that is
+ * not -inf: of codes whose K was smoothed (tb_quant_per_block_int8 with mean) the
+ * lse then is that of the scores against K itself.  q, q_scale, lse and strides (elements, 3
+ * values: q b, h, l) as for tb_sparse_attn; key_mean [B, Hk, D] of type mean_dtype
+ * (BF16 / F16), contiguous, 16-byte aligned; D = 128. */
+TB_API int tb_smoothed_lse(const int8_t *q, const float *q_scale, const void *key_mean,
+                           int mean_dtype, float *lse, int64_t B, int64_t Hq, int64_t Hk,
+                           int64_t Lq, int64_t D, const int64_t *strides, float sm_scale,
+                           tb_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -574,6 +574,93 @@ def test_rotary_choice_and_attention_together(layout):
     check(out, lse, ref, torch.bfloat16, keep * 64, layout)
 
 
+def shifted(n, L, dtype, layout, seed, D=128):
+    """Keys whose channels have means far from zero, as smoothing is for."""
+    k = value(2, n, L, torch.float32, layout, seed, D)
+    g = torch.Generator().manual_seed(seed + 100)
+    return (k + 3.0 * torch.randn(D, generator=g).cuda()).to(dtype)
+
+
+def token_mean(k, layout):
+    return to_hnd(k, layout).double().mean(dim=2).float().to(k.dtype)
+
+
+def mean_scores(pre, mean, layout, sm_scale):
+    """sm_scale q . mean and its bound in fp32: 128 products summed."""
+    q = dequant(pre.query_int8, pre.query_scale, 16, layout)
+    mean = torch.nn.functional.pad(mean, (0, 128 - mean.size(-1))).double()
+    mean = mean.repeat_interleave(q.size(1) // mean.size(1), dim=1)[:, :, None]
+    return (q * mean).sum(dim=3) * sm_scale, (q * mean).abs().sum(dim=3) * abs(sm_scale) * 132 * 2.0 ** -24
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("layout,D,Lq,keep", [("HND", 128, 300, 5), ("NHD", 128, 1, 12),
+                                              ("NHD", 96, 130, 1000)])
+def test_lse_of_smoothed_keys(dtype, layout, D, Lq, keep):
+    """The lse counts the mean that smoothing took off K, row by row; of a row that
+    sees no key it stays -inf.  The output and its lists do not change."""
+    q = value(2, 4, Lq, dtype, layout, 1, D)
+    k, v = shifted(2, 900, dtype, layout, 2, D), value(2, 2, 900, dtype, layout, 3, D)
+    lens = [900, 0]
+    key_lengths = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    kw = dict(key_lengths=key_lengths, return_lse=True)
+    out, lse = turing_sage.sparse_sageattn(q, k, v, keep, tensor_layout=layout, smooth_k=True,
+                                           **kw)
+    pre = turing_sage.prequantize_sageattn(q, k, v, tensor_layout=layout, smooth_k=True)
+    lists = turing_sage.select_key_blocks(pre.query_int8, pre.query_scale, pre.key_int8,
+                                          pre.key_scale, keep, tensor_layout=layout,
+                                          key_lengths=key_lengths)
+    codes_ = (pre.query_int8, pre.query_scale, pre.key_int8, pre.key_scale, pre.value)
+    o, A, want = reference(*codes_, lists, layout, lens, sm_scale=D ** -0.5)
+    check(out, None, (o[..., :D], A[..., :D], want), dtype, 900, layout)
+    shift, slack = mean_scores(pre, token_mean(k, layout), layout, D ** -0.5)
+    assert (lse[1] == -math.inf).all()
+    err = (lse.double() - want - shift).abs()[0]
+    lim = (5.3e-4 + 2.0 ** -22 * want.abs() + 2.0 ** -23 * (want + shift).abs() + slack)[0]
+    assert shift.abs().max() > 1 and (err <= lim).all(), (err - lim).max().item()
+    # The same in parts, and without smoothing as before.
+    again = turing_sage.sparse_sageattn_from_prequantized(pre, keep, **kw)
+    assert torch.equal(again[0], out) and torch.equal(again[1], lse)
+    parts = turing_sage.sparse_sageattn_prequantized(
+        *codes_, lists, tensor_layout=layout, sm_scale=D ** -0.5, key_mean=pre.key_mean, **kw)
+    assert torch.equal(parts[1], lse)
+    plain = turing_sage.sparse_sageattn_prequantized(*codes_, lists, tensor_layout=layout,
+                                                     sm_scale=D ** -0.5, **kw)
+    assert torch.equal(parts[0], plain[0])
+    assert ((plain[1].double() - want).abs()[0] <= 5.3e-4 + 2.0 ** -22 * want.abs()[0]).all()
+    assert turing_sage.prequantize_sageattn(q, k, v, tensor_layout=layout).key_mean is None
+
+
+@gpu
+def test_smoothed_halves_join_by_their_lse():
+    """Two halves of the keys, each smoothed by its own mean, joined by their lse:
+    the attention over all keys.  Joining weights two outputs by e^lse: an lse off by
+    e moves their share by at most 2 e, so the output by 2 e (|o1| + |o2|)."""
+    q = value(2, 2, 200, torch.bfloat16, "HND", 1)
+    parts, scores, values, outs, slacks = [], [], [], [], []
+    for seed in (2, 3):
+        k, v = shifted(2, 320, torch.bfloat16, "HND", seed), value(2, 2, 320, torch.bfloat16,
+                                                                   "HND", seed + 5)
+        outs.append(turing_sage.sparse_sageattn(q, k, v, 5, smooth_k=True, return_lse=True))
+        pre = turing_sage.prequantize_sageattn(q, k, v, smooth_k=True)
+        shift, slack = mean_scores(pre, token_mean(k, "HND"), "HND", 128 ** -0.5)
+        s = dequant(pre.query_int8, pre.query_scale, 16, "HND") @ dequant(
+            pre.key_int8, pre.key_scale, 64, "HND").transpose(2, 3) * 128 ** -0.5
+        scores.append(s + shift[..., None])
+        values.append(v.double())
+        slacks.append(slack)
+    w = torch.cat(scores, dim=3).softmax(dim=3)
+    want, A = w @ torch.cat(values, dim=2), w @ torch.cat(values, dim=2).abs()
+    lses = torch.stack([x[1].double() for x in outs])
+    share = lses.softmax(dim=0)[..., None]
+    got = sum(share[i] * outs[i][0].double() for i in range(2))
+    e = 5.3e-4 + 2.0 ** -21 * lses.abs().max() + torch.stack(slacks).amax(dim=0)
+    size = outs[0][0].double().abs() + outs[1][0].double().abs()
+    bound = (2.0 ** -8 + 5.3e-4) * A + 2.0 ** -8 * size + 2 * e[..., None] * size
+    assert ((got - want).abs() <= bound).all(), ((got - want).abs() - bound).max().item()
+
+
 @gpu
 @pytest.mark.parametrize("Lq", [1, 300])
 def test_graphs_streams_and_compile(Lq):
@@ -763,4 +850,45 @@ def test_c_entry_refusals():
                      (dict(sm=float("nan")), "sm_scale"), (dict(B=1 << 20, Hq=1 << 20), "grid"),
                      (dict(strides=(8,) * 12), "multiples of 16"), (dict(strides=(0,) * 6 + (4,) * 6), "V/O")):
         assert attend(**kw) == _lib.TB_ERR_INVALID, kw
+        assert text in _lib.last_error(), (kw, _lib.last_error())
+
+
+@pytest.mark.parametrize("mean", [fake(2, 4, 128, dtype=torch.float16),
+                                  fake(2, 2, 64, dtype=torch.float16),
+                                  fake(2, 2, 128, dtype=torch.float32),
+                                  torch.zeros((2, 2, 128), dtype=torch.float16)])
+def test_key_mean_refusals(mean):
+    with pytest.raises(RuntimeError, match="key_mean"):
+        turing_sage.sparse_sageattn_prequantized(
+            **good(), v=fake(2, 2, 200, 128, dtype=torch.float16),
+            block_index=fake(2, 4, 2, 3, dtype=torch.int32), key_mean=mean)
+
+
+def test_lse_of_anchored_keys_is_refused():
+    """stabilize_k takes a row off K that the codes do not keep."""
+    from comfyui_turing_utils_kernel.turing_sage.core import (PrequantizedQK,
+                                                              prequantize_sageattn_from_qk)
+
+    cpu, x = torch.zeros((1, 1, 8, 128), dtype=torch.int8), torch.zeros((1, 1, 8, 128)).half()
+    qk = PrequantizedQK(cpu, torch.ones((1, 1, 4)), cpu, torch.ones((1, 1, 1)), "HND", x.dtype,
+                        128, True, True)
+    with pytest.raises(ValueError, match="stabilize_k"):
+        turing_sage.sparse_sageattn_from_prequantized(prequantize_sageattn_from_qk(qk, x), 1,
+                                                      return_lse=True)
+
+
+def test_smoothed_lse_entry_refusals():
+    lib, p, odd = _lib.load(), ctypes.c_void_p(4096), ctypes.c_void_p(4100)
+
+    def add(q=p, mean=p, dtype=0, B=1, Hq=2, Hk=1, Lq=128, D=128, sm=1.0, stride=0):
+        return lib.tb_smoothed_lse(q, p, mean, dtype, p, B, Hq, Hk, Lq, D,
+                                   (ctypes.c_int64 * 3)(*((stride,) * 3)), sm, None)
+
+    for kw, text in ((dict(q=None), "CUDA tensors"), (dict(mean=None), "CUDA tensors"),
+                     (dict(q=odd), "16-byte"), (dict(mean=odd), "16-byte"), (dict(D=64), "head_dim"),
+                     (dict(dtype=2), "float16 or bfloat16"), (dict(Lq=0), "empty"),
+                     (dict(Hk=0), "divisible"), (dict(Hq=3, Hk=2), "divisible"),
+                     (dict(sm=float("inf")), "sm_scale"), (dict(stride=8), "multiples of 16"),
+                     (dict(B=1 << 20, Hq=1 << 20), "grid")):
+        assert add(**kw) == _lib.TB_ERR_INVALID, kw
         assert text in _lib.last_error(), (kw, _lib.last_error())
