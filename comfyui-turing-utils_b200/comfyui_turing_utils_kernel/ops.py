@@ -11,6 +11,7 @@ from __future__ import annotations
 import math
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 from torch.utils._python_dispatch import is_in_torch_dispatch_mode
 
 from . import _C
@@ -387,6 +388,14 @@ def turing_rope_inv_freq(
     return torch.cat(freqs).to(device), scale
 
 
+def _refuse_tangents(*tensors):
+    """A registered op has no forward-mode rule and would drop the tangent."""
+    if forward_ad._current_level >= 0 and any(
+            forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("the registered rotary ops have no forward-mode derivative; call "
+                           "turing_rope or turing_rope_qk")
+
+
 @torch.library.custom_op("turing_utils::rope", mutates_args=())
 def _rope_op(
     x: torch.Tensor,
@@ -399,6 +408,7 @@ def _rope_op(
     inverse: bool = False,
 ) -> torch.Tensor:
     _require_cuda(x, "Rotary positions")
+    _refuse_tangents(x)
     return _C.turing_rope(x, None, positions, inv_freq, tensor_layout, split_half, axis_pairs,
                           scale, inverse)[0]
 
@@ -422,6 +432,7 @@ def _rope_qk_op(
     inverse: bool = False,
 ) -> tuple[torch.Tensor, torch.Tensor]:
     _require_cuda(query, "Rotary positions")
+    _refuse_tangents(query, key)
     return _C.turing_rope(query, key, positions, inv_freq, tensor_layout, split_half, axis_pairs,
                           scale, inverse)
 
@@ -465,14 +476,25 @@ _rope_qk_op.register_autograd(_rope_qk_backward, setup_context=_rope_setup)
 # Eager calls on plain CUDA tensors skip the custom op's dispatcher, which costs
 # more than a small launch (one token: 68 us a call through it against 21, with
 # its gradients 289 against 140): without gradients they reach the binding, with
-# gradients by way of an autograd function.  Tracing (torch.compile, fake and
-# subclass tensors, dispatch modes) sees the custom op.
+# gradients by way of an autograd function.  Tracing (torch.compile, torch.jit,
+# fake and subclass tensors, dispatch modes) sees the custom op.  Function
+# transforms (torch.func, torch.vmap) and forward-mode differentiation, whose
+# wrapped tensors have the plain type, go through _RopeTransformed.
 
 _PLAIN = (torch.Tensor, torch.nn.Parameter)
 
 
+_function_transforms_active = torch._C._are_functorch_transforms_active
+_jit_tracing = torch._C._is_tracing
+
+
+def _transformed() -> bool:
+    return _function_transforms_active() or forward_ad._current_level >= 0
+
+
 def _eager(*tensors: torch.Tensor) -> bool:
-    if torch.compiler.is_compiling() or is_in_torch_dispatch_mode():
+    if (torch.compiler.is_compiling() or is_in_torch_dispatch_mode() or _transformed()
+            or _jit_tracing()):
         return False
     return all(type(t) in _PLAIN and t.is_cuda for t in tensors)
 
@@ -504,6 +526,48 @@ class _RopeFunction(torch.autograd.Function):
         return grad_query, grad_key, None, None, None
 
 
+class _Options:
+    """Options of a call as one opaque argument (a tuple would be taken apart)."""
+
+    def __init__(self, values):
+        self.values = values
+
+
+def _rope_registered(query, key, positions, inv_freq, options):
+    if key is None:
+        return _rope_op(query, positions, inv_freq, *options)
+    return _rope_qk_op(query, key, positions, inv_freq, *options)
+
+
+class _RopeTransformed(torch.autograd.Function):
+    """The rotation under function transforms: linear in query and key, so the
+    tangent is the rotated tangent; batched by the registered ops' rule."""
+
+    generate_vmap_rule = True
+
+    @staticmethod
+    def forward(query, key, positions, inv_freq, options):
+        return _rope_registered(query, key, positions, inv_freq, options.values)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        _, key, positions, inv_freq, options = inputs
+        ctx.save_for_backward(positions, inv_freq)
+        ctx.save_for_forward(positions, inv_freq)
+        ctx.pair, ctx.options = key is not None, options
+
+    @staticmethod
+    def backward(ctx, grad_query, grad_key=None):
+        values = ctx.options.values
+        back = _Options((*values[:-1], not values[-1]))
+        grads = _RopeTransformed.apply(grad_query, grad_key, *ctx.saved_tensors, back)
+        return (*(grads if ctx.pair else (grads, None)), None, None, None)
+
+    @staticmethod
+    def jvp(ctx, query, key, *_):
+        return _RopeTransformed.apply(query, key, *ctx.saved_tensors, ctx.options)
+
+
 def _rope_call(query, key, positions, inv_freq, options):
     if _eager(query, positions, inv_freq) if key is None else _eager(query, key, positions,
                                                                      inv_freq):
@@ -512,9 +576,9 @@ def _rope_call(query, key, positions, inv_freq, options):
             return _RopeFunction.apply(query, key, positions, inv_freq, options)
         rotated = _C.turing_rope(query, key, positions, inv_freq, *options)
         return rotated[0] if key is None else rotated
-    if key is None:
-        return _rope_op(query, positions, inv_freq, *options)
-    return _rope_qk_op(query, key, positions, inv_freq, *options)
+    if not torch.compiler.is_compiling() and _transformed():
+        return _RopeTransformed.apply(query, key, positions, inv_freq, _Options(options))
+    return _rope_registered(query, key, positions, inv_freq, options)
 
 
 def turing_rope(

@@ -303,6 +303,62 @@ def test_c_entry_in_place(split_half):
         assert torch.equal(y, want)
 
 
+def transforms(x, pos, inv):
+    """What torch's function transforms, forward-mode differentiation and the tracer
+    give for a rotation, against the rotation itself (linear: its tangent is the
+    rotated tangent, its gradient the inverse rotation)."""
+    import torch.autograd.forward_ad as fwd
+
+    rope = lambda t: kernel.turing_rope(t, pos, inv, split_half=True)  # noqa: E731
+    both = lambda t: kernel.turing_rope_qk(t, 2 * t, pos, inv)         # noqa: E731
+    y = rope(x)
+    many = torch.stack([x, x + 1, -x])
+    assert torch.equal(torch.vmap(rope)(many), torch.stack([rope(t) for t in many]))
+    assert torch.equal(torch.vmap(both)(many)[1], torch.stack([both(t)[1] for t in many]))
+    shifts = torch.stack([pos, pos + 3, pos * 2])
+    assert torch.equal(torch.vmap(lambda t, p: kernel.turing_rope(t, p, inv))(many, shifts),
+                       torch.stack([kernel.turing_rope(t, p, inv) for t, p in zip(many, shifts)]))
+    loss = lambda t: (rope(t) ** 2).sum() / 2                          # noqa: E731
+    back = kernel.turing_rope(y, pos, inv, split_half=True, inverse=True)
+    assert torch.equal(torch.func.grad(loss)(x), back)
+    assert torch.equal(torch.vmap(torch.func.grad(loss))(many)[0], back)
+    grads = torch.func.grad(lambda q, k: sum((t ** 2).sum() / 2 for t in
+                                             kernel.turing_rope_qk(q, k, pos, inv)),
+                            argnums=(0, 1))(x, x + 1)
+    leaves = [t.clone().requires_grad_() for t in (x, x + 1)]
+    out = kernel.turing_rope_qk(*leaves, pos, inv)
+    want = torch.autograd.grad(out, leaves, [t.detach() for t in out])
+    assert all(torch.equal(a, b) for a, b in zip(grads, want))
+    tangent = (x * 3 + 1).detach()
+    assert torch.equal(torch.func.jvp(rope, (x,), (tangent,))[1], rope(tangent))
+    with fwd.dual_level():
+        primal, t = fwd.unpack_dual(rope(fwd.make_dual(x, tangent)))
+        assert torch.equal(primal, y) and torch.equal(t, rope(tangent))
+        q, k = kernel.turing_rope_qk(fwd.make_dual(x, tangent), x, pos, inv)
+        assert torch.equal(fwd.unpack_dual(q).tangent, kernel.turing_rope(tangent, pos, inv))
+        assert torch.equal(kernel.turing_rope(x, pos, inv, split_half=True), y)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.ops.turing_utils.rope(fwd.make_dual(x, tangent), pos, inv)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.ops.turing_utils.rope_qk(x, fwd.make_dual(x, tangent), pos, inv)
+    second = torch.func.hessian(loss)(x[:1, :1])
+    n = x[:1, :1].numel()
+    eye = second.reshape(n, n)      # a rotation of scale 1: the identity
+    assert (eye - torch.eye(n, dtype=eye.dtype, device=eye.device)).abs().max() <= 4e-6
+    traced = torch.jit.trace(rope, (x,))
+    assert torch.equal(traced(many[1]), rope(many[1]))
+    traced = torch.jit.trace(lambda p: kernel.turing_rope_freqs(p, inv, dtype=torch.float32), (pos,))
+    assert torch.equal(traced(pos + 5), kernel.turing_rope_freqs(pos + 5, inv, dtype=torch.float32))
+
+
+@gpu
+@pytest.mark.filterwarnings("ignore")
+def test_function_transforms():
+    x = rand((2, 3, 5, 8), "HND", torch.float32, 1)
+    inv, _ = kernel.turing_rope_inv_freq(8, device="cuda")
+    transforms(x, torch.arange(5, device="cuda"), inv)
+
+
 # ---------------------------------------------------------------------- CPU --
 
 def test_fake_contracts():
@@ -315,6 +371,35 @@ def test_fake_contracts():
     assert kernel.turing_rope(q.transpose(1, 2), pos, inv).is_contiguous()
     f = kernel.turing_rope_freqs(pos, inv, axis_pairs=[12, 10, 10], dtype=torch.float16)
     assert f.shape == (1, 9, 1, 32, 2, 2) and f.dtype == torch.float16
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_function_transforms_without_a_gpu(monkeypatch):
+    """The same through the registered ops, the formula in the kernels' place."""
+    from comfyui_turing_utils_kernel import ops
+
+    def plain(query, key, positions, inv_freq, layout, split_half, axis_pairs, scale, inverse):
+        sign = -1.0 if inverse else 1.0
+        outs = []
+        for t in (query, key):
+            t = None if t is None else t.contiguous()
+            assert t is None or t.data_ptr()      # a tensor with memory of its own
+            outs.append(None if t is None else formula(t, positions, inv_freq, layout, split_half,
+                                                       axis_pairs, scale, sign)[0].to(t.dtype))
+        return tuple(outs)
+
+    def matrices(positions, inv_freq, axis_pairs, scale, dtype):
+        assert positions.data_ptr()
+        ang = angles(positions, inv_freq, axis_pairs)
+        c, s = ang.cos() * scale, ang.sin() * scale
+        return torch.stack([c, -s, s, c], dim=-1).view(*ang.shape[:2], 1, -1, 2, 2).to(dtype)
+
+    monkeypatch.setattr(ops._C, "turing_rope", plain)
+    monkeypatch.setattr(ops._C, "turing_rope_freqs", matrices)
+    monkeypatch.setattr(ops, "_require_cuda", lambda *a: None)
+    x = torch.randn((2, 3, 5, 8), generator=torch.Generator().manual_seed(1))
+    inv, _ = kernel.turing_rope_inv_freq(8)
+    transforms(x, torch.arange(5), inv)
 
 
 def test_inv_freq():
