@@ -581,6 +581,12 @@ def _rope_call(query, key, positions, inv_freq, options):
     return _rope_registered(query, key, positions, inv_freq, options)
 
 
+def _options(tensor_layout, split_half, axis_pairs, scale, inverse):
+    # A list of its own: the gradients use it after the caller may have changed theirs.
+    return (tensor_layout, split_half, None if axis_pairs is None else list(axis_pairs),
+            float(scale), inverse)
+
+
 def turing_rope(
     x: torch.Tensor,
     positions: torch.Tensor,
@@ -604,8 +610,8 @@ def turing_rope(
     reach positions and inv_freq.  To capture a backward pass into a CUDA graph,
     take leaves that no live eager graph holds (torch raises an error otherwise).
     """
-    return _rope_call(x, None, positions, inv_freq,
-                      (tensor_layout, split_half, axis_pairs, float(scale), inverse))
+    return _rope_call(x, None, positions, inv_freq, _options(
+        tensor_layout, split_half, axis_pairs, scale, inverse))
 
 
 def turing_rope_qk(
@@ -622,8 +628,8 @@ def turing_rope_qk(
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """turing_rope of query and key (same batch, length and head dimension, any
     head counts) in one launch, differentiable in both."""
-    return _rope_call(query, key, positions, inv_freq,
-                      (tensor_layout, split_half, axis_pairs, float(scale), inverse))
+    return _rope_call(query, key, positions, inv_freq, _options(
+        tensor_layout, split_half, axis_pairs, scale, inverse))
 
 
 @torch.library.custom_op("turing_utils::rope_freqs", mutates_args=())

@@ -359,6 +359,22 @@ def test_function_transforms():
     transforms(x, torch.arange(5, device="cuda"), inv)
 
 
+@gpu
+@pytest.mark.parametrize("op", [False, True])
+def test_axis_pairs_changed_after_the_call(op):
+    """The gradient turns by the axes of the call, whatever becomes of its list."""
+    pos = torch.arange(12, device="cuda").view(6, 2)
+    inv, _ = kernel.turing_rope_inv_freq(16, device="cuda")
+    x, g = (rand((1, 2, 6, 16), "HND", torch.float32, s) for s in (1, 2))
+    x.requires_grad_()
+    want, = torch.autograd.grad(kernel.turing_rope(x, pos, inv, axis_pairs=[3, 5]), x, g)
+    pairs = [3, 5]
+    y = (torch.ops.turing_utils.rope if op else kernel.turing_rope)(x, pos, inv, axis_pairs=pairs)
+    pairs[:] = [6, 2]
+    got, = torch.autograd.grad(y, x, g)
+    assert torch.equal(got, want)
+
+
 # ---------------------------------------------------------------------- CPU --
 
 def test_fake_contracts():
