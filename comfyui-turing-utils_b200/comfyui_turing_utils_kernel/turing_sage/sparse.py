@@ -44,7 +44,7 @@ def select_key_blocks(q_int8: torch.Tensor, q_scale: torch.Tensor, k_int8: torch
     dequantized query and key; the `keep` highest are taken, ties to the lowest
     block, a NaN score last.  The mean query is held to 2^-40 of its largest
     channel, all else is exact up to one fp64 rounding; a query block with a scale
-    that is not finite scores 0 everywhere.  Positive sm_scale, K smoothing and
+    that is not finite scores 0 everywhere, a key block with one comes last.  Positive sm_scale, K smoothing and
     the Hadamard rotation change no rank beyond INT8 rounding.
 
     q_int8 / k_int8 and scales: as the Sage quantizers return them (head_dim 64 or

@@ -7,7 +7,8 @@
 // which ranks as the mean score of the pair's query-key grid does (sm_scale and
 // the query count change no rank), and the `keep` blocks of the highest score
 // in ascending order, ties to the lowest block.  block_policy takes a block out
-// (-1) or ranks it above every score (1); a NaN score ranks lowest.
+// (-1) or ranks it above every score (1); a NaN score, as under a k_scale that is
+// not finite, ranks lowest.
 //
 // Which of two near blocks is kept is decided by the last digits, so the dot
 // product is integer: qm_i is rounded to 40 bits below the power of two above
@@ -226,7 +227,10 @@ __global__ void __launch_bounds__(kSumThreads, 8) block_sums_kernel(const Select
       *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
       if (D < kChannels) *reinterpret_cast<uint4*>(dst + D) = make_uint4(0, 0, 0, 0);
     }
-    if (lane == 0) p.k_factor[at] = static_cast<double>(scale) / n;
+    // Under an infinite scale the dequantized keys are infinities of both signs and
+    // 0 * inf: the block's mean is no number, as under a NaN.
+    if (lane == 0)
+      p.k_factor[at] = isfinite(scale) ? static_cast<double>(scale) / n : static_cast<double>(NAN);
     return;
   }
   int i, bh;

@@ -458,8 +458,8 @@ TB_API int tb_rope_freqs(const void *positions, int position_type, int64_t posit
  * the product of the mean dequantized query and the mean dequantized visible
  * key (the mean query held to 2^-40 of its largest channel, all else exact up to
  * one fp64 rounding; a query block with a scale that is not finite scores 0
- * everywhere); the keep highest are taken, ties to the lowest block, a NaN
- * score last.  q, k: the INT8 codes of the Sage quantizers with q_scale
+ * everywhere, a key block with one comes last); the keep highest are taken, ties
+ * to the lowest block, a NaN score last.  q, k: the INT8 codes of the Sage quantizers with q_scale
  * [B, Hq, ceil(Lq/64)*4] and k_scale [B, Hk, ceil(Lk/64)]; strides (elements,
  * 6 values): q (b, h, l), k (b, h, l), multiples of 16, last dimension
  * contiguous, Q/K 16-byte aligned.  key_lengths int32 [B] or NULL: keys from

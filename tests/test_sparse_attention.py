@@ -458,6 +458,22 @@ def test_choice_over_long_contexts(Lk, keep):
 
 
 @gpu
+@pytest.mark.parametrize("Lk", [100000, 200000])
+def test_nan_and_infinite_scales_over_long_contexts(Lk):
+    """Keys beyond the part of a row that the search holds in registers: a NaN score
+    comes last and an infinite one first or last, wherever its block lies."""
+    q8, qs = codes(1, 1, 150, 128, 16, "HND", 1)
+    k8, ks = codes(1, 1, Lk, 128, 64, "HND", 2)
+    for at in (0, 1400, -1):
+        ks[0, 0, at] = float("nan")
+        ks[0, 0, at - 2] = float("inf")
+    n = ks.size(2)
+    for keep in (1, 9, n - 2):
+        got = turing_sage.select_key_blocks(q8, qs, k8, ks, keep)
+        assert torch.equal(got, choose(q8, qs, k8, ks, keep, "HND"))
+
+
+@gpu
 def test_choice_reads_views():
     """Codes as views of a fused row (16-byte aligned strides, not contiguous)."""
     g = torch.Generator().manual_seed(1)
