@@ -641,55 +641,79 @@ __global__ void __launch_bounds__(kCombineWarps * 32) sparse_combine_kernel(cons
 
 // lse += sm_scale * q_scale * (Q8 . mean) of each row: the part of every score that
 // K smoothing took off (the scores of the codes are those against K - mean).  Eight
-// lanes a row, 16 channels each; the products are exact in fp32.  Bound by the bytes
-// of Q8 and the lse.
+// lanes a row, 16 channels each, whose means stay in registers over 16 rows; the
+// products are exact in fp32.  Bound by the latency of its loads and shuffles:
+// 75600 queries x 40 heads 130 us (3.2 TB/s; four rows in flight, for which fewer
+// warps fit, 148).
 constexpr int kShiftThreads = 256;
 constexpr int kShiftLanes = kDim / 16;
+constexpr int kShiftStep = kShiftThreads / kShiftLanes;  // rows of a CTA at a time
+constexpr int kShiftRows = 16 * kShiftStep;
+
+// Byte i of x plus 128, minus 128, as a float: exact, and off the conversion unit.
+// x: the four codes with their sign bits turned.
+__device__ __forceinline__ float code_f32(uint32_t x, int i) {
+  return __uint_as_float(__byte_perm(x, 0x4b000000u, 0x7440 + i)) - 8388736.0f;
+}
 
 template <typename TM>
-__global__ void __launch_bounds__(kShiftThreads)
+__global__ void __launch_bounds__(kShiftThreads, 5)
     smoothed_lse_kernel(const int8_t* q, int64_t q_sb, int64_t q_sh, int64_t q_sl,
-                        const float* q_scale, const TM* mean, float* lse, int64_t rows, int Hq,
+                        const float* q_scale, const TM* mean, float* lse, int chunks, int Hq,
                         int Lq, int groups, int q_tiles_scale, float sm_scale) {
-  const int64_t flat =
-      static_cast<int64_t>(blockIdx.x) * (kShiftThreads / kShiftLanes) + threadIdx.x / kShiftLanes;
+  const int bh = static_cast<int>(blockIdx.x) / chunks;
+  const int row0 = static_cast<int>(blockIdx.x) % chunks * kShiftRows + threadIdx.x / kShiftLanes;
   const int part = threadIdx.x % kShiftLanes;
-  float sum = 0.0f;
-  int bh = 0, row = 0;
-  if (flat < rows) {
-    bh = static_cast<int>(flat / Lq);
-    row = static_cast<int>(flat - static_cast<int64_t>(bh) * Lq);
-    const int b = bh / Hq, h = bh % Hq;
-    const uint4 x = *reinterpret_cast<const uint4*>(q + b * q_sb + h * q_sh + row * q_sl +
-                                                    part * 16);
-    const uint4* m = reinterpret_cast<const uint4*>(
-        mean + static_cast<int64_t>(b * (Hq / groups) + h / groups) * kDim + part * 16);
-    const uint4 m0 = __ldg(m), m1 = __ldg(m + 1);
-    const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
-    const uint32_t mw[8] = {m0.x, m0.y, m0.z, m0.w, m1.x, m1.y, m1.z, m1.w};
+  const int b = bh / Hq, h = bh % Hq;
+  const uint4* m = reinterpret_cast<const uint4*>(
+      mean + static_cast<int64_t>(b * (Hq / groups) + h / groups) * kDim + part * 16);
+  const uint4 m0 = __ldg(m), m1 = __ldg(m + 1);
+  const uint32_t mw[8] = {m0.x, m0.y, m0.z, m0.w, m1.x, m1.y, m1.z, m1.w};
+  float mv[16];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float lo, hi;
-      if constexpr (std::is_same<TM, __nv_bfloat16>::value) {
-        lo = __uint_as_float(mw[i] << 16);
-        hi = __uint_as_float(mw[i] & 0xffff0000u);
-      } else {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&mw[i]));
-        lo = f.x;
-        hi = f.y;
-      }
-      const uint32_t two = xw[i / 2] >> (16 * (i & 1));
-      sum = fmaf(static_cast<float>(static_cast<int8_t>(two)), lo, sum);
-      sum = fmaf(static_cast<float>(static_cast<int8_t>(two >> 8)), hi, sum);
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (std::is_same<TM, __nv_bfloat16>::value) {
+      mv[2 * i] = __uint_as_float(mw[i] << 16);
+      mv[2 * i + 1] = __uint_as_float(mw[i] & 0xffff0000u);
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&mw[i]));
+      mv[2 * i] = f.x;
+      mv[2 * i + 1] = f.y;
     }
   }
+  const int8_t* src = q + b * q_sb + h * q_sh + part * 16;
+  const float* scales = q_scale + static_cast<int64_t>(bh) * q_tiles_scale;
+  float* out = lse + static_cast<int64_t>(bh) * Lq;
+  constexpr int kFly = 2;  // rows in flight
+#pragma unroll 1
+  for (int r0 = row0; r0 < row0 + kShiftRows; r0 += kFly * kShiftStep) {
+    uint4 x[kFly];
+    float scale[kFly], old[kFly];
 #pragma unroll
-  for (int i = kShiftLanes / 2; i > 0; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
-  if (flat < rows && part == 0) {
-    const float scale =
-        sm_scale * __ldg(q_scale + static_cast<int64_t>(bh) * q_tiles_scale + row / 16);
-    // A row that saw no key stays -inf.
-    if (lse[flat] != -INFINITY) lse[flat] = fmaf(scale, sum, lse[flat]);
+    for (int u = 0; u < kFly; ++u) {
+      const int r = r0 + u * kShiftStep;
+      x[u] = make_uint4(0u, 0u, 0u, 0u);
+      scale[u] = old[u] = 0.0f;
+      if (r < Lq) {
+        x[u] = *reinterpret_cast<const uint4*>(src + r * q_sl);
+        scale[u] = __ldg(scales + r / 16);
+        old[u] = out[r];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kFly; ++u) {
+      const uint32_t w[4] = {x[u].x ^ 0x80808080u, x[u].y ^ 0x80808080u, x[u].z ^ 0x80808080u,
+                             x[u].w ^ 0x80808080u};
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sum = fmaf(code_f32(w[i / 4], i & 3), mv[i], sum);
+#pragma unroll
+      for (int i = kShiftLanes / 2; i > 0; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
+      const int r = r0 + u * kShiftStep;
+      // A row that saw no key stays -inf.
+      if (part == 0 && r < Lq && old[u] != -INFINITY)
+        out[r] = fmaf(sm_scale * scale[u], sum, old[u]);
+    }
   }
 }
 
@@ -845,15 +869,14 @@ extern "C" int tb_smoothed_lse(const int8_t* q, const float* q_scale, const void
     for (int i = 0; i < 3; ++i)
       TB_REQUIRE(strides[i] % 16 == 0, "Q strides must be multiples of 16 bytes");
     require_sm100();
-    const int64_t rows = B * Hq * Lq;
-    constexpr int kRowsCta = kShiftThreads / kShiftLanes;
-    const int64_t ctas = (rows + kRowsCta - 1) / kRowsCta;
-    TB_REQUIRE(ctas <= INT32_MAX, "batch, heads and queries exceed the grid range");
+    const int64_t chunks = (Lq + kShiftRows - 1) / kShiftRows;
+    TB_REQUIRE(B * Hq * chunks <= INT32_MAX, "batch, heads and queries exceed the grid range");
     auto launch = [&](auto kern, auto* mean) {
-      kern<<<static_cast<unsigned>(ctas), kShiftThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-          q, strides[0], strides[1], strides[2], q_scale, mean, lse, rows, static_cast<int>(Hq),
-          static_cast<int>(Lq), static_cast<int>(Hq / Hk), static_cast<int>((Lq + 63) / 64 * 4),
-          sm_scale);
+      kern<<<static_cast<unsigned>(B * Hq * chunks), kShiftThreads, 0,
+             static_cast<cudaStream_t>(stream)>>>(
+          q, strides[0], strides[1], strides[2], q_scale, mean, lse, static_cast<int>(chunks),
+          static_cast<int>(Hq), static_cast<int>(Lq), static_cast<int>(Hq / Hk),
+          static_cast<int>((Lq + 63) / 64 * 4), sm_scale);
       TB_CUDA_CHECK(cudaGetLastError());
     };
     if (mean_dtype == TB_DTYPE_BF16)

@@ -612,7 +612,7 @@ def mean_scores(pre, mean, layout, sm_scale):
 @gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("layout,D,Lq,keep", [("HND", 128, 300, 5), ("NHD", 128, 1, 12),
-                                              ("NHD", 96, 130, 1000)])
+                                              ("NHD", 96, 130, 1000), ("HND", 64, 1100, 2)])
 def test_lse_of_smoothed_keys(dtype, layout, D, Lq, keep):
     """The lse counts the mean that smoothing took off K, row by row; of a row that
     sees no key it stays -inf.  The output and its lists do not change."""
