@@ -604,8 +604,8 @@ def turing_rope(
     The first 2 * len(inv_freq) channels of each head turn; the others are
     copied.  Pair p, channels (2p, 2p + 1) or with split_half (p, p + pairs),
     turns by position * inv_freq[p] (the angle is taken in fp64) and is
-    multiplied by scale.  positions: int32, int64 (within 2^51), float32 or
-    float64, [L] or [1 or B, L]; with axis_pairs (pairs of each of 1 to 4 axes)
+    multiplied by scale.  positions: int32, int64, float32 or float64, within 2^51
+    in magnitude as their products with inv_freq, [L] or [1 or B, L]; with axis_pairs (pairs of each of 1 to 4 axes)
     [L, axes] or [1 or B, L, axes].  inverse turns the other way.  No gradients
     reach positions and inv_freq.  To capture a backward pass into a CUDA graph,
     take leaves that no live eager graph holds (torch raises an error otherwise).

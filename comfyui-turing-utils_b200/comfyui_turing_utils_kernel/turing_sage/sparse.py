@@ -43,7 +43,7 @@ def select_key_blocks(q_int8: torch.Tensor, q_scale: torch.Tensor, k_int8: torch
     The score of a query block and a key block is the product of their mean
     dequantized query and key; the `keep` highest are taken, ties to the lowest
     block, a NaN score last.  The mean query is held to 2^-40 of its largest
-    channel, all else is exact up to one fp64 rounding; a query block with a scale
+    channel, all else is exact up to three fp64 roundings; a query block with a scale
     that is not finite scores 0 everywhere, a key block with one comes last.  Positive sm_scale, K smoothing and
     the Hadamard rotation change no rank beyond INT8 rounding.
 

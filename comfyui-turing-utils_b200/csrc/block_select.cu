@@ -14,8 +14,8 @@
 // product is integer: qm_i is rounded to 40 bits below the power of two above
 // its largest channel and written as six digits of base 128 in [-64, 63], S_j
 // (14 bits) as two, and the tensor core multiplies the digit planes exactly
-// (kind::i8, INT32 sums below 2^20).  The planes join in 64-bit integers, and
-// the product with k_scale_j / n_j is the first fp64 rounding.  The sum order
+// (kind::i8, INT32 sums below 2^20).  The planes join in 64-bit integers.  fp64
+// rounds the sum (past 2^53), k_scale_j / n_j and their product.  The sum order
 // never matters, equal blocks score equal.
 //
 //   1. block_sums_kernel: 16-byte loads, channel sums by dp4a of transposed
@@ -29,7 +29,10 @@
 //      and 4-7 take the tiles in turn and leave the top word of each score's
 //      sortable bits in shared memory.  Then one warp per query block finds the
 //      keep-th word (choose_row), and, where that word is shared by more blocks
-//      than fit, again with their low words from the digits.  Two CTAs per SM
+//      than fit, again with their low words from the digits, one block after the
+//      other: rare, but a query block of zeros (padding) ties all blocks (one such
+//      among 1182 key blocks: 1.0 ms in all; 30 of 591 in each of 40 heads 1.4 ms,
+//      0.38 without; 24576 key blocks 19 ms).  Two CTAs per SM
 //      (up to 1300 key blocks): one's search runs under the other's products.
 //      Bound by the latency of the scores' read-back and of the search, not by the
 //      tensor core: 75600 tokens x 40 heads, 1182 key blocks: 174 us, after 136 us
@@ -800,8 +803,11 @@ void check_select(int64_t B, int64_t Hq, int64_t Hk, int64_t Lq, int64_t Lk, int
 void select_launch(SelectParams& p, cudaStream_t stream) {
   // Query blocks per CTA: fewer where their keys outgrow shared memory or where
   // the CTAs would not fill the SMs (the search is a warp per query block, the
-  // products of idle rows cost nothing that matters).  8 heads, 8 query blocks, 313
-  // key blocks: 8.5 us, 9.4 with full CTAs; 12 heads, 33, 73: 7.5 and 7.2.
+  // products of idle rows cost nothing that matters).  Where the SMs would not fill,
+  // sums included, by the rule and with full CTAs (heads x query blocks, key blocks):
+  // 1 x 591, 1182: 18.8 and 22.2 us; 8 x 8, 313: 13.2 and 14.0; 1 x 8, 313: 10.0 and
+  // 10.9; 5 x 118, 236: 12.6 and 12.9; 12 x 33, 73: the same; the other way 40 x 2, 128:
+  // 14.5 and 14.4; 2 x 256, 512: 15.2 and 14.2.
   const int64_t head_rows = static_cast<int64_t>(p.Hq) / p.Hk * p.query_blocks;
   const int64_t heads = static_cast<int64_t>(p.B) * p.Hk;
   auto smem_of = [&](int rows) {

@@ -426,7 +426,8 @@ TB_API int tb_w8a8_attn(const int8_t *q, const int8_t *k, const void *v_codes,
  * (p, p + rot_dim / 2), turns by position * inv_freq[p] (fp64 [rot_dim / 2]),
  * by the negative angle when inverse != 0 (the gradient), and is multiplied by
  * scale.  positions: contiguous [position_batches, length, axes] of type
- * TB_POS_* (I64: within 2^51), position_batches 1 (shared) or batch; axis_pairs (host, int32
+ * TB_POS_* (within 2^51 in magnitude, as their products with inv_freq: past it
+ * fp64 has no phase left), position_batches 1 (shared) or batch; axis_pairs (host, int32
  * [axes], or NULL for one axis) counts the pairs that turn with each axis.
  * strides (elements, 12 values): query (b, h, l), key (b, h, l), query_out
  * (b, h, l), key_out (b, h, l); the last dimension is contiguous.  Any
@@ -457,7 +458,7 @@ TB_API int tb_rope_freqs(const void *positions, int position_type, int64_t posit
  * filled up with -1 where fewer blocks can be chosen.  The score of a pair is
  * the product of the mean dequantized query and the mean dequantized visible
  * key (the mean query held to 2^-40 of its largest channel, all else exact up to
- * one fp64 rounding; a query block with a scale that is not finite scores 0
+ * three fp64 roundings; a query block with a scale that is not finite scores 0
  * everywhere, a key block with one comes last); the keep highest are taken, ties
  * to the lowest block, a NaN score last.  q, k: the INT8 codes of the Sage quantizers with q_scale
  * [B, Hq, ceil(Lq/64)*4] and k_scale [B, Hk, ceil(Lk/64)]; strides (elements,

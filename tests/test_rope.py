@@ -1,9 +1,10 @@
 """Rotary positions: the fp64 formula, gradients, refusals, frequencies.
 
 Bound of one output y = s (x0 cos - x1 sin) in fp32 against fp64: the reduced
-angle is rounded to half turns in [-1, 1] (2^-25 pi = 0.94e-7), its sine and
-cosine are good to 2 ulp (1.2e-7), the scale, the product and the sum round once
-each (3 x 0.6e-7): 4e-7 s (|x0| + |x1|); then half a step of the output type.
+angle, quarter turns in [-1/2, 1/2], is rounded once (2^-26 pi / 2 = 0.23e-7), the
+polynomials of its sine and cosine are good to 1 ulp of values up to 1 (0.6e-7; 2
+are allowed for), the scale, the product and the sum round once each (3 x 0.6e-7):
+3.3e-7 s (|x0| + |x1|), 4e-7 allowed; then half a step of the output type.
 """
 from __future__ import annotations
 
