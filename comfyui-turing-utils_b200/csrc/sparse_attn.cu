@@ -645,7 +645,7 @@ __global__ void __launch_bounds__(kCombineWarps * 32) sparse_combine_kernel(cons
 // K smoothing took off (the scores of the codes are those against K - mean).  Eight
 // lanes a row, 16 channels each, whose means stay in registers over 16 rows; the
 // products are exact in fp32.  Bound by the latency of its loads and shuffles:
-// 75600 queries x 40 heads 130 us (3.2 TB/s; four rows in flight, for which fewer
+// 75600 queries x 40 heads 137 us (3.0 TB/s; four rows in flight, for which fewer
 // warps fit, 148).
 constexpr int kShiftThreads = 256;
 constexpr int kShiftLanes = kDim / 16;
@@ -664,7 +664,9 @@ __global__ void __launch_bounds__(kShiftThreads, 5)
                         const float* q_scale, const TM* mean, float* lse, int chunks, int Hq,
                         int Lq, int groups, int q_tiles_scale, float sm_scale) {
   const int bh = static_cast<int>(blockIdx.x) / chunks;
-  const int row0 = static_cast<int>(blockIdx.x) % chunks * kShiftRows + threadIdx.x / kShiftLanes;
+  // Unsigned: rows past the last one are counted past 2^31 in the longest sequences.
+  const uint32_t row0 =
+      blockIdx.x % static_cast<uint32_t>(chunks) * kShiftRows + threadIdx.x / kShiftLanes;
   const int part = threadIdx.x % kShiftLanes;
   const int b = bh / Hq, h = bh % Hq;
   const uint4* m = reinterpret_cast<const uint4*>(
@@ -688,15 +690,15 @@ __global__ void __launch_bounds__(kShiftThreads, 5)
   float* out = lse + static_cast<int64_t>(bh) * Lq;
   constexpr int kFly = 2;  // rows in flight
 #pragma unroll 1
-  for (int r0 = row0; r0 < row0 + kShiftRows; r0 += kFly * kShiftStep) {
+  for (uint32_t r0 = row0; r0 < row0 + kShiftRows; r0 += kFly * kShiftStep) {
     uint4 x[kFly];
     float scale[kFly], old[kFly];
 #pragma unroll
     for (int u = 0; u < kFly; ++u) {
-      const int r = r0 + u * kShiftStep;
+      const uint32_t r = r0 + u * kShiftStep;
       x[u] = make_uint4(0u, 0u, 0u, 0u);
       scale[u] = old[u] = 0.0f;
-      if (r < Lq) {
+      if (r < static_cast<uint32_t>(Lq)) {
         x[u] = *reinterpret_cast<const uint4*>(src + r * q_sl);
         scale[u] = __ldg(scales + r / 16);
         old[u] = out[r];
@@ -711,9 +713,9 @@ __global__ void __launch_bounds__(kShiftThreads, 5)
       for (int i = 0; i < 16; ++i) sum = fmaf(code_f32(w[i / 4], i & 3), mv[i], sum);
 #pragma unroll
       for (int i = kShiftLanes / 2; i > 0; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
-      const int r = r0 + u * kShiftStep;
+      const uint32_t r = r0 + u * kShiftStep;
       // A row that saw no key stays -inf.
-      if (part == 0 && r < Lq && old[u] != -INFINITY)
+      if (part == 0 && r < static_cast<uint32_t>(Lq) && old[u] != -INFINITY)
         out[r] = fmaf(sm_scale * scale[u], sum, old[u]);
     }
   }
